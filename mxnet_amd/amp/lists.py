@@ -13,7 +13,7 @@ FP16_FUNCS = [
 # keep in fp32 (reductions / exponentials with wide dynamic range)
 FP32_FUNCS = [
     'softmax', 'log_softmax', 'SoftmaxOutput', 'norm', 'mean', 'sum',
-    'exp', 'log', 'BatchNorm', 'LayerNorm', 'erf', 'erfinv',
+    'exp', 'log', 'BatchNorm', 'LayerNorm', 'RMSNorm', 'erf', 'erfinv',
 ]
 
 # run in the widest input type

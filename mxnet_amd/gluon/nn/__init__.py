@@ -1,8 +1,8 @@
 from ..block import (Block, HybridBlock, SymbolBlock, Sequential,
                      HybridSequential)
 from .basic_layers import (Dense, Dropout, BatchNorm, BatchNormReLU,
-                           SyncBatchNorm, Embedding, LayerNorm, GroupNorm,
-                           InstanceNorm, Flatten, Activation, Lambda,
+                           SyncBatchNorm, Embedding, LayerNorm, RMSNorm,
+                           GroupNorm, InstanceNorm, Flatten, Activation, Lambda,
                            HybridLambda, Identity)
 from .conv_layers import (Conv1D, Conv2D, Conv3D, Conv1DTranspose,
                           Conv2DTranspose, MaxPool2D, AvgPool2D,

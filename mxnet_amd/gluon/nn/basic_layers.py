@@ -272,6 +272,34 @@ class LayerNorm(HybridBlock):
         return super().cast(dtype)
 
 
+class RMSNorm(HybridBlock):
+    """Root-mean-square norm of the last axis; called with a residual it
+    adds it first and returns ``[norm, sum]`` (one kernel for both)."""
+
+    def __init__(self, axis=-1, epsilon=1e-6, gamma_initializer='ones',
+                 in_channels=0, **kwargs):
+        super().__init__(**kwargs)
+        self._axis = axis
+        self._epsilon = epsilon
+        self.gamma = Parameter('gamma', shape=(in_channels,),
+                               init=init.create(gamma_initializer),
+                               allow_deferred_init=True)
+
+    def infer_shape(self, x, residual=None):
+        self.gamma.shape = (x.shape[self._axis],)
+
+    def hybrid_forward(self, F, x, residual=None, gamma=None):
+        return F.RMSNorm(x, gamma, residual=residual, axis=self._axis,
+                         eps=self._epsilon)
+
+    def cast(self, dtype):
+        """gamma stays fp32 under half-precision training, as LayerNorm's
+        does: the kernel multiplies in fp32."""
+        if dtype in ('float16', 'bfloat16'):
+            return self
+        return super().cast(dtype)
+
+
 class GroupNorm(HybridBlock):
     def __init__(self, num_groups=1, epsilon=1e-5, center=True, scale=True,
                  in_channels=0, **kwargs):

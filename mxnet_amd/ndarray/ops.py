@@ -187,6 +187,38 @@ def LayerNorm(data, gamma, beta, axis=-1, eps=1e-5, **kwargs):
     return NDArray(_nn.layer_norm(_t(data), _t(gamma), _t(beta), axis, eps))
 
 
+def RMSNorm(data, gamma, residual=None, axis=-1, eps=1e-6, out_type=None,
+            **kwargs):
+    """Root-mean-square norm of the last axis, with the residual's addition.
+
+    ``h = data + residual`` (rounded to the data's type),
+    ``y = h / sqrt(mean(h ** 2) + eps) * gamma``.  Returns ``y``, or
+    ``[y, h]`` with a residual: h is the next residual, and gradients flow
+    through both.  With ``out_type='int8'`` (inference) y is given as
+    ``q * scale``, int8 values and one float32 scale a row, for an int8
+    product: ``[q, scale]`` or ``[q, scale, h]``.  A row of zeros has a scale
+    of 1; a row that holds a NaN or an infinity has one of NaN.
+    """
+    if data.is_native:
+        if axis not in (-1, data.ndim - 1):
+            raise NotImplementedError('RMSNorm only over the last axis')
+        if out_type not in (None, 'int8'):
+            raise ValueError(f'RMSNorm: out_type must be None or int8, got '
+                             f'{out_type!r}')
+        ins = [data, gamma] + ([residual] if residual is not None else [])
+        attrs = {'eps': repr(float(eps))}
+        if out_type == 'int8':
+            outs = _ninv('_contrib_rms_norm_int8', ins, attrs, nout=3)
+            return outs if residual is not None else outs[:2]
+        outs = _ninv('RMSNorm', ins, attrs, nout=3)
+        return outs[:2] if residual is not None else outs[0]
+    out = _nn.rms_norm(_t(data), _t(gamma),
+                       _t(residual) if residual is not None else None, axis,
+                       eps, out_type)
+    return [NDArray(o) for o in out] if isinstance(out, tuple) \
+        else NDArray(out)
+
+
 def Embedding(data, weight, input_dim=None, output_dim=None, dtype=None,
               sparse_grad=False, **kwargs):
     if data.is_native:

@@ -8,7 +8,7 @@ from .util import set_np, reset_np, is_np_array  # noqa: F401
 
 __all__ = ['set_np', 'reset_np', 'is_np_array', 'softmax', 'log_softmax',
            'masked_softmax', 'relu', 'sigmoid', 'gelu', 'batch_norm',
-           'layer_norm', 'fully_connected', 'convolution', 'pooling',
+           'layer_norm', 'rms_norm', 'fully_connected', 'convolution', 'pooling',
            'embedding', 'one_hot', 'pick', 'topk', 'batch_dot',
            'sequence_mask', 'gamma', 'erf']
 
@@ -19,6 +19,7 @@ sigmoid = lambda x: NDArray(torch.sigmoid(x._t))
 gelu = lambda x: NDArray(torch.nn.functional.gelu(x._t, approximate='tanh'))
 batch_norm = _ops.BatchNorm
 layer_norm = _ops.LayerNorm
+rms_norm = _ops.RMSNorm
 fully_connected = _ops.FullyConnected
 convolution = _ops.Convolution
 pooling = _ops.Pooling

@@ -405,6 +405,40 @@ def layernorm_bwd(dy, x, gamma, mean, istd):
     return [dx, dgamma.to(gamma.dtype), dbeta.to(gamma.dtype)]
 
 
+def rms_norm_fwd(x, gamma, residual, eps, int8=False):
+    """(y, sum or None, rstd), or with int8 (q, sum or None, scale); the
+    statistic keeps the leading axes, with a last one of 1."""
+    x = _c(x)
+    dev, s = _dev_stream(x)
+    y = torch.empty(x.shape, dtype=torch.int8 if int8 else x.dtype,
+                    device=x.device)
+    stat = torch.empty(x.shape[:-1] + (1,), dtype=torch.float32,
+                       device=x.device)
+    res = _c(residual) if residual is not None else None
+    total = torch.empty_like(x) if res is not None else None
+    st = _arr(stat)
+    _raw.rms_norm_fwd(dev, s, _arr(x), _arr(_f32(gamma)), _arr(res), eps,
+                      _arr(y), st if int8 else None, _arr(total),
+                      None if int8 else st)
+    return y, total, stat
+
+
+def rms_norm_bwd(dy, dsum, h, gamma, rstd):
+    dy, h = _c(dy), _c(h)
+    dev, s = _dev_stream(h)
+    C = h.shape[-1]
+    rows = h.numel() // C
+    dx = torch.empty_like(h)
+    dgamma = torch.empty((C,), dtype=torch.float32, device=h.device)
+    partial = torch.empty((_raw.rms_norm_bwd_blocks(rows), C),
+                          dtype=torch.float32, device=h.device)
+    _raw.rms_norm_bwd(dev, s, _arr(dy),
+                      _arr(_c(dsum)) if dsum is not None else None, _arr(h),
+                      _arr(_f32(gamma)), _arr(rstd), _arr(dx), _arr(dgamma),
+                      _arr(partial))
+    return dx, dgamma.to(gamma.dtype)
+
+
 # ---------------------------------------------------------------------------
 # pooling
 # ---------------------------------------------------------------------------

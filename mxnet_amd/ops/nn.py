@@ -594,6 +594,97 @@ def layer_norm(x, gamma, beta, axis=-1, eps=1e-5):
     return y.to(x.dtype)
 
 
+class _RMSNorm(torch.autograd.Function):
+    """Fused (residual addition +) root-mean-square norm of the last axis;
+    both outputs are differentiable."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, residual, eps):
+        ext = hip_required('rms_norm')
+        y, total, rstd = ext.rms_norm_fwd(x, gamma, residual, eps)
+        ctx.save_for_backward(total if residual is not None else x, gamma,
+                              rstd)
+        ctx.set_materialize_grads(False)
+        return y if residual is None else (y, total)
+
+    @staticmethod
+    def backward(ctx, dy, dsum=None):
+        h, gamma, rstd = ctx.saved_tensors
+        if dy is None:  # only the sum was used
+            return dsum, None, dsum, None
+        dx, dgamma = hip_required('rms_norm').rms_norm_bwd(dy, dsum, h,
+                                                           gamma, rstd)
+        return dx, dgamma, dx if ctx.needs_input_grad[2] else None, None
+
+
+def _rms_norm_check(x, gamma, residual, out_type):
+    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f'RMSNorm: float16, bfloat16 or float32 data, got '
+                        f'{x.dtype}')
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError('RMSNorm: data needs a last axis to norm')
+    if gamma.dim() != 1 or gamma.shape[0] != x.shape[-1] \
+            or not gamma.is_floating_point():
+        raise ValueError(f'RMSNorm: gamma must hold one value for each of '
+                         f'{x.shape[-1]} columns, got {tuple(gamma.shape)} '
+                         f'{gamma.dtype}')
+    if residual is not None and (residual.shape != x.shape
+                                 or residual.dtype != x.dtype):
+        raise ValueError(f'RMSNorm: the residual must be like the data, '
+                         f'{tuple(x.shape)} {x.dtype}, got '
+                         f'{tuple(residual.shape)} {residual.dtype}')
+    for t in (gamma, residual):
+        if t is not None and t.device != x.device:
+            raise ValueError(f'RMSNorm: data on {x.device}, another input on '
+                             f'{t.device}')
+    if out_type not in (None, 'int8'):
+        raise ValueError(f'RMSNorm: out_type must be None or int8, got '
+                         f'{out_type!r}')
+
+
+def rms_norm(x, gamma, residual=None, axis=-1, eps=1e-6, out_type=None):
+    """y = h / sqrt(mean(h^2) + eps) * gamma over the last axis, h = x +
+    residual.  Returns y, or (y, h) with a residual; with ``out_type='int8'``
+    (q, scale) or (q, scale, h), where q * scale stands for y."""
+    if axis not in (-1, x.dim() - 1):
+        raise NotImplementedError('rms_norm only over the last axis')
+    _rms_norm_check(x, gamma, residual, out_type)
+    if out_type == 'int8':
+        if torch.is_grad_enabled() and any(
+                t is not None and t.requires_grad
+                for t in (x, gamma, residual)):
+            raise ValueError('RMSNorm: the int8 output has no gradient; call '
+                             'it outside autograd.record() or on detached '
+                             'arrays')
+        if use_hip(x) and x.numel():
+            q, h, scale = hip_required('rms_norm').rms_norm_fwd(
+                x, gamma, residual, eps, int8=True)
+            return (q, scale) if h is None else (q, scale, h)
+    elif use_hip(x) and x.numel():
+        return _RMSNorm.apply(x.contiguous(), gamma,
+                              None if residual is None
+                              else residual.contiguous(), eps)
+    h = x if residual is None else x + residual
+    hf = h.float()
+    r = (1.0 / torch.sqrt(hf.double().square().mean(-1, keepdim=True)
+                          + eps)).float()
+    y = hf * r * gamma.float()
+    if out_type is None:
+        y = y.to(x.dtype)
+        return y if residual is None else (y, h)
+    top = y.abs().amax(-1, keepdim=True) if y.numel() \
+        else y.new_zeros(y.shape[:-1] + (1,))
+    inv = torch.reciprocal(top) * 127.0
+    some = (top > 0) & ~torch.isinf(inv)
+    scale = torch.where(some, top * (1.0 / 127.0), torch.ones_like(top))
+    q = torch.round(y * torch.where(some, inv, torch.zeros_like(top)))
+    # a row with a NaN or an infinity has no scale
+    bad = ~torch.isfinite(hf).all(-1, keepdim=True)
+    scale = scale.masked_fill(bad, float('nan'))
+    q = q.masked_fill(bad, 0.0).clamp(-127, 127).to(torch.int8)
+    return (q, scale) if residual is None else (q, scale, h)
+
+
 # ---------------------------------------------------------------------------
 # Embedding / Dropout
 # ---------------------------------------------------------------------------

@@ -382,3 +382,15 @@ _OP_NAMES = [
 ]
 for _n in _OP_NAMES:
     globals().setdefault(_n, _make_op(_n))
+
+
+def RMSNorm(data, gamma, residual=None, axis=-1, eps=1e-6, out_type=None,
+            name=None):
+    """nd.RMSNorm as a graph node: one Symbol, or a list of them where
+    nd.RMSNorm returns a list."""
+    kw = {} if residual is None else {'residual': residual}
+    y = _make_op('RMSNorm')(data, gamma, name=name, axis=axis, eps=eps,
+                            out_type=out_type, **kw)
+    n = 1 + (residual is not None) + (out_type == 'int8')
+    y._node.num_outputs = n
+    return y if n == 1 else [Symbol(y._node, i) for i in range(n)]

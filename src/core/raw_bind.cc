@@ -41,6 +41,26 @@ LaunchCtx MakeLC(int dev, uintptr_t stream) {
   return lc;
 }
 
+// launch context of ops whose callers bring every buffer: no arena, and the
+// tensors' device is the current one for the launch
+struct Launch {
+  int before = -1;
+  LaunchCtx lc;
+  Launch(int dev, uintptr_t stream) {
+    lc.stream = (hipStream_t)stream;
+    lc.dev = dev;
+    int cur = 0;
+    MX_HIP_CALL(hipGetDevice(&cur));
+    if (cur != dev) {
+      MX_HIP_CALL(hipSetDevice(dev));
+      before = cur;
+    }
+  }
+  ~Launch() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
 }  // namespace
 
 void init_raw(py::module_& m) {
@@ -159,6 +179,23 @@ void init_raw(py::module_& m) {
                       ToArr(dbeta));
   });
 
+  r.def("rms_norm_fwd", [](int dev, uintptr_t stream, py::handle x,
+                           py::handle gamma, py::handle residual, double eps,
+                           py::handle y, py::handle scale, py::handle sum,
+                           py::handle rstd) {
+    Launch l(dev, stream);
+    rms_norm_fwd_raw(l.lc, ToArr(x), ToArr(gamma), ToArr(residual), eps,
+                     ToArr(y), ToArr(scale), ToArr(sum), ToArr(rstd));
+  });
+  r.def("rms_norm_bwd_blocks", &rms_norm_bwd_blocks);
+  r.def("rms_norm_bwd", [](int dev, uintptr_t stream, py::handle dy,
+                           py::handle dsum, py::handle h, py::handle gamma,
+                           py::handle rstd, py::handle dx, py::handle dgamma,
+                           py::handle partial) {
+    Launch l(dev, stream);
+    rms_norm_bwd_raw(l.lc, ToArr(dy), ToArr(dsum), ToArr(h), ToArr(gamma),
+                     ToArr(rstd), ToArr(dx), ToArr(dgamma), ToArr(partial));
+  });
   r.def("conv2d_fwd", [](int dev, uintptr_t stream, py::handle x,
                          py::handle w, py::handle bias, int sh, int sw,
                          int ph, int pw, int dh, int dw, int groups,

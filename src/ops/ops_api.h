@@ -71,6 +71,18 @@ void layernorm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& x,
                        const Arr& gamma, const Arr& mean, const Arr& rstd,
                        const Arr& dx, const Arr& dgamma, const Arr& dbeta);
 
+// ---- rmsnorm.hip ----------------------------------------------------------
+// h = x (+ residual, written to sum); y = h * rstd * gamma, or int8 with one
+// scale a row where y's dtype is int8 (then rstd is not written)
+void rms_norm_fwd_raw(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
+                      const Arr& residual, double eps, const Arr& y,
+                      const Arr& scale, const Arr& sum, const Arr& rstd);
+// partial: fp32 workspace of rms_norm_bwd_blocks(rows) * C values
+int64_t rms_norm_bwd_blocks(int64_t rows);
+void rms_norm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
+                      const Arr& h, const Arr& gamma, const Arr& rstd,
+                      const Arr& dx, const Arr& dgamma, const Arr& partial);
+
 // ---- conv.hip (NHWC) ------------------------------------------------------
 void conv2d_fwd_raw(const LaunchCtx& lc, const Arr& x, const Arr& w,
                     const Arr& bias, int sh, int sw, int ph, int pw, int dh,

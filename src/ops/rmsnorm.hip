@@ -1,0 +1,577 @@
+// Root-mean-square norm over the last axis, with the residual's addition in
+// front and an int8 output with one scale a row.
+//
+//   h = data + residual                (rounded to the data's type: it is
+//                                       stored, and the norm is of what is)
+//   r = 1 / sqrt(mean(h^2) + eps)
+//   y = h * r * gamma
+//   int8: a = max|y|, scale = a * (1 / 127), q = rint(y * (127 * (1 / a))),
+//         each factor rounded to 32 bits
+//
+//   backward, from dy and the sum's own gradient dsum:
+//   g = dy * gamma, n = h * r
+//   dh = r * (g - n * mean(g * n)) + dsum      (for data and residual alike)
+//   dgamma = sum over rows of dy * n
+//
+// Both directions are bound by HBM: about ten operations for eight bytes
+// moved.  So a row is read once and stays in registers between its sum and
+// its output: a wave a row where it fits (no barrier at all), else a block.
+// The sum of squares is held in 64 bits.  It costs no time here (64-bit FMAs
+// run at the rate of 32-bit ones, far under the memory's time) and makes r
+// the correctly rounded value, so that an int8 step does not depend on the
+// order in which a row's squares were added.
+#include "ops_api.h"
+
+namespace mxcore {
+namespace {
+
+DEV_INLINE double wave_sum_f64(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// sum over the TPR threads of a row; `red` holds one value a wave.  The two
+// barriers keep a second call from overwriting what a slow wave still reads.
+template <int TPR>
+DEV_INLINE double row_sum(double v, double* red) {
+  v = wave_sum_f64(v);
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) v += red[i];
+    __syncthreads();
+  }
+  return v;
+}
+
+template <int TPR>
+DEV_INLINE float row_sum_f32(float v, float* red) {
+  v = wave_reduce_sum(v);
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) v += red[i];
+    __syncthreads();
+  }
+  return v;
+}
+
+template <int TPR>
+DEV_INLINE float row_max(float v, float* red) {
+  v = wave_reduce_max(v);
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) v = fmaxf(v, red[i]);
+    __syncthreads();
+  }
+  return v;
+}
+
+DEV_INLINE float inv_rms(double sumsq, int C, double eps) {
+  return (float)(1.0 / sqrt(sumsq / C + eps));
+}
+
+// a row's scale and its reciprocal.  A row of zeros (or so small that
+// 127 / a overflows) quantises to zeros under a scale of 1; a row that holds
+// a NaN or an infinity has a sum that is not finite, and a scale of NaN.
+DEV_INLINE void int8_scale(float a, double sumsq, float* scale, float* inv) {
+  *scale = a * (1.0f / 127.0f);
+  *inv = 127.0f * (1.0f / a);
+  if (!(a > 0.f) || isinf(*inv)) {
+    *scale = 1.f;
+    *inv = 0.f;
+  }
+  if (!isfinite(sumsq)) {
+    *scale = __builtin_nanf("");
+    *inv = 0.f;
+  }
+}
+
+DEV_INLINE signed char to_int8(float v) {
+  float q = rintf(v);
+  q = q > 127.f ? 127.f : q < -127.f ? -127.f : q;
+  return q == q ? (signed char)q : (signed char)0;
+}
+
+// ---------------------------------------------------------------------------
+// forward, the row in registers: TPR threads a row, NV vectors a thread
+// ---------------------------------------------------------------------------
+template <typename T, int VEC, int TPR, int NV, bool RES, bool INT8>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
+    const T* __restrict__ x, const T* __restrict__ res,
+    const float* __restrict__ gamma, T* __restrict__ y,
+    signed char* __restrict__ q, float* __restrict__ scale,
+    T* __restrict__ sum, float* __restrict__ rstd, long rows, int C,
+    double eps) {
+  using VecT = T __attribute__((ext_vector_type(VEC)));
+  using VecG = float __attribute__((ext_vector_type(VEC)));
+  using VecQ = signed char __attribute__((ext_vector_type(VEC)));
+  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+  __shared__ double red[TPR > 64 ? TPR / 64 : 1];
+  const int lane = threadIdx.x % TPR;
+  const long row = (long)blockIdx.x * RPB + threadIdx.x / TPR;
+  if (row >= rows) return;  // whole waves, and only where no barrier follows
+  const long base = row * C;
+  VecT h[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + lane) * VEC;
+    if (c < C) h[i] = *(const VecT*)(x + base + c);
+  }
+  double s = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + lane) * VEC;
+    if (c < C) {
+      if constexpr (RES) {
+        const VecT r = *(const VecT*)(res + base + c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) h[i][j] = (T)((float)h[i][j] + (float)r[j]);
+        *(VecT*)(sum + base + c) = h[i];
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const double f = (double)(float)h[i][j];
+        s += f * f;
+      }
+    }
+  }
+  s = row_sum<TPR>(s, red);
+  const float r = inv_rms(s, C, eps);
+  if (!INT8 && lane == 0) rstd[row] = r;
+  if constexpr (!INT8) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < C) {
+        const VecG g = *(const VecG*)(gamma + c);
+        VecT o;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = (T)((float)h[i][j] * r * g[j]);
+        *(VecT*)(y + base + c) = o;
+      }
+    }
+  } else {
+    float v[NV][VEC];
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < C) {
+        const VecG g = *(const VecG*)(gamma + c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[i][j] = (float)h[i][j] * r * g[j];
+          a = fmaxf(a, fabsf(v[i][j]));
+        }
+      }
+    }
+    a = row_max<TPR>(a, (float*)red);
+    float sc, inv;
+    int8_scale(a, s, &sc, &inv);
+    if (lane == 0) scale[row] = sc;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < C) {
+        VecQ o;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = to_int8(v[i][j] * inv);
+        *(VecQ*)(q + base + c) = o;
+      }
+    }
+  }
+}
+
+// forward of rows that no register variant holds: the row is read again, from
+// the cache
+template <typename T, bool RES, bool INT8>
+__global__ __launch_bounds__(1024) void rms_fwd_long_kernel(
+    const T* __restrict__ x, const T* __restrict__ res,
+    const float* __restrict__ gamma, T* __restrict__ y,
+    signed char* __restrict__ q, float* __restrict__ scale,
+    T* __restrict__ sum, float* __restrict__ rstd, long rows, int C,
+    double eps) {
+  __shared__ double red[16];
+  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const long base = row * C;
+    auto value = [&](int c) {
+      const float f = (float)x[base + c];
+      return RES ? (float)(T)(f + (float)res[base + c]) : f;
+    };
+    double s = 0;
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      const double f = value(c);
+      s += f * f;
+    }
+    s = row_sum<1024>(s, red);
+    const float r = inv_rms(s, C, eps);
+    if (!INT8 && threadIdx.x == 0) rstd[row] = r;
+    float sc = 0.f, inv = 0.f;
+    if constexpr (INT8) {
+      float a = 0.f;
+      for (int c = threadIdx.x; c < C; c += 1024)
+        a = fmaxf(a, fabsf(value(c) * r * gamma[c]));
+      a = row_max<1024>(a, (float*)red);
+      int8_scale(a, s, &sc, &inv);
+      if (threadIdx.x == 0) scale[row] = sc;
+    }
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      const float f = value(c);
+      if constexpr (RES) sum[base + c] = (T)f;
+      if constexpr (INT8)
+        q[base + c] = to_int8(f * r * gamma[c] * inv);
+      else
+        y[base + c] = (T)(f * r * gamma[c]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// backward, one pass over dy, h (and dsum): a thread keeps its columns for
+// all rows of its block, so dgamma's partial sums stay in registers; the
+// blocks' partials are added by rms_dgamma_kernel in a fixed order.
+// ---------------------------------------------------------------------------
+template <typename T, int VEC, int TPR, int NV, bool DSUM>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
+    const T* __restrict__ dy, const T* __restrict__ dsum,
+    const T* __restrict__ h, const float* __restrict__ gamma,
+    const float* __restrict__ rstd, T* __restrict__ dx,
+    float* __restrict__ partial, long rows, int C) {
+  using VecT = T __attribute__((ext_vector_type(VEC)));
+  using VecG = float __attribute__((ext_vector_type(VEC)));
+  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  float dg[NV][VEC] = {};
+  for (long row = (long)blockIdx.x * RPB + sub; row < rows;
+       row += (long)gridDim.x * RPB) {
+    const long base = row * C;
+    const float r = rstd[row];
+    VecT a[NV], b[NV], e[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < C) {
+        a[i] = *(const VecT*)(dy + base + c);
+        b[i] = *(const VecT*)(h + base + c);
+        if constexpr (DSUM) e[i] = *(const VecT*)(dsum + base + c);
+      }
+    }
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < C) {
+        const VecG g = *(const VecG*)(gamma + c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float d = (float)a[i][j], n = (float)b[i][j] * r;
+          m += d * g[j] * n;
+          dg[i][j] += d * n;
+        }
+      }
+    }
+    m = row_sum_f32<TPR>(m, red) / C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < C) {
+        const VecG g = *(const VecG*)(gamma + c);
+        VecT o;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          float v = r * ((float)a[i][j] * g[j] - (float)b[i][j] * r * m);
+          if constexpr (DSUM) v += (float)e[i][j];
+          o[j] = (T)v;
+        }
+        *(VecT*)(dx + base + c) = o;
+      }
+    }
+  }
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (c < C)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          partial[(long)blockIdx.x * C + c + j] = dg[i][j];
+    }
+  } else {
+    __shared__ float part[RPB][TPR * NV * VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        part[sub][(i * TPR + lane) * VEC + j] = dg[i][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < C; c += 256) {
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < RPB; ++k) v += part[k][c];
+      partial[(long)blockIdx.x * C + c] = v;
+    }
+  }
+}
+
+template <typename T, bool DSUM>
+__global__ __launch_bounds__(1024) void rms_bwd_long_kernel(
+    const T* __restrict__ dy, const T* __restrict__ dsum,
+    const T* __restrict__ h, const float* __restrict__ gamma,
+    const float* __restrict__ rstd, T* __restrict__ dx, long rows, int C) {
+  __shared__ float red[16];
+  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const long base = row * C;
+    const float r = rstd[row];
+    float m = 0.f;
+    for (int c = threadIdx.x; c < C; c += 1024)
+      m += (float)dy[base + c] * gamma[c] * ((float)h[base + c] * r);
+    m = row_sum_f32<1024>(m, red) / C;
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      float v = r * ((float)dy[base + c] * gamma[c] -
+                     (float)h[base + c] * r * m);
+      if constexpr (DSUM) v += (float)dsum[base + c];
+      dx[base + c] = (T)v;
+    }
+  }
+}
+
+// a thread a column over one block row's share of the rows
+template <typename T>
+__global__ __launch_bounds__(256) void rms_dgamma_long_kernel(
+    const T* __restrict__ dy, const T* __restrict__ h,
+    const float* __restrict__ rstd, float* __restrict__ partial, long rows,
+    int C) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= C) return;
+  float v = 0.f;
+  for (long row = blockIdx.y; row < rows; row += gridDim.y)
+    v += (float)dy[row * C + c] * ((float)h[row * C + c] * rstd[row]);
+  partial[(long)blockIdx.y * C + c] = v;
+}
+
+// dgamma[c] = sum of the partials' column c: 64 columns a block, 16 threads a
+// column, always in the same order
+__global__ __launch_bounds__(1024) void rms_dgamma_kernel(
+    const float* __restrict__ partial, float* __restrict__ dgamma, int nblk,
+    int C) {
+  __shared__ float part[16][64];
+  const int col = threadIdx.x & 63, k = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + col;
+  float v = 0.f;
+  if (c < C)
+    for (int b = k; b < nblk; b += 16) v += partial[(long)b * C + c];
+  part[k][col] = v;
+  __syncthreads();
+  if (k == 0 && c < C) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += part[i][col];
+    dgamma[c] = v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// which variant: the smallest number of threads whose registers hold the row
+// (a wave a row needs no barrier, but a launch of few rows wants the whole
+// block on each, or most of the chip idles)
+// ---------------------------------------------------------------------------
+struct RowPlan {
+  int tpr = 0, nv = 0;  // 0: the kernel that reads the row again
+  bool vec = false;     // 16-byte accesses
+};
+
+RowPlan plan_rows(long rows, int C, size_t size, bool aligned) {
+  RowPlan p;
+  const int vec = aligned && (C * size) % 16 == 0 ? (int)(16 / size) : 1;
+  p.vec = vec > 1;
+  auto fits = [&](int tpr, int nv) {
+    if (p.tpr == 0 && C <= (long)tpr * nv * vec) {
+      p.tpr = tpr;
+      p.nv = nv;
+    }
+  };
+  if (p.vec) {
+    if (rows >= 1024 || C <= 64 * vec) {
+      fits(64, 1);
+      fits(64, 2);
+      fits(64, 4);
+    }
+    fits(256, 1);
+    fits(256, 2);
+    fits(256, 4);
+    fits(1024, 4);
+  } else {
+    fits(64, 4);
+    fits(256, 4);
+    fits(256, 16);
+    fits(1024, 16);
+  }
+  return p;
+}
+
+#define RMS_CASE(VEC_, TPR_, NV_) \
+  if (p.vec == (VEC_ > 1) && p.tpr == TPR_ && p.nv == NV_) { \
+    constexpr int VEC = VEC_, TPR = TPR_, NV = NV_; \
+    LAUNCH(); \
+    return; \
+  }
+
+// LAUNCH sees VEC, TPR and NV as constants
+#define RMS_DISPATCH(FULL) \
+  RMS_CASE(FULL, 64, 1) \
+  RMS_CASE(FULL, 64, 2) \
+  RMS_CASE(FULL, 64, 4) \
+  RMS_CASE(FULL, 256, 1) \
+  RMS_CASE(FULL, 256, 2) \
+  RMS_CASE(FULL, 256, 4) \
+  RMS_CASE(FULL, 1024, 4) \
+  RMS_CASE(1, 64, 4) \
+  RMS_CASE(1, 256, 4) \
+  RMS_CASE(1, 256, 16) \
+  RMS_CASE(1, 1024, 16)
+
+bool aligned16(std::initializer_list<const void*> ps) {
+  for (auto p : ps)
+    if ((uintptr_t)p & 15) return false;
+  return true;
+}
+
+void check_rows(const Arr& x, const Arr& gamma, const char* name) {
+  MX_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < (1 << 30),
+           name << ": the last axis must have 1 to 2^30 - 1 elements");
+  MX_CHECK(gamma.dtype == kFloat32 && gamma.numel() == x.size(-1),
+           name << ": gamma must be float32, one value a column");
+  MX_CHECK(x.numel() / x.size(-1) < (1L << 31),
+           name << ": 2^31 rows or more");
+}
+
+template <typename T, bool RES, bool INT8>
+void fwd_launch(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
+                const Arr& res, double eps, const Arr& y, const Arr& scale,
+                const Arr& sum, const Arr& rstd) {
+  const int C = (int)x.size(-1);
+  const long rows = x.numel() / C;
+  RowPlan p = plan_rows(rows, C, sizeof(T),
+                        aligned16({x.ptr, gamma.ptr, y.ptr, res.ptr,
+                                   sum.ptr}));
+  T* yp = INT8 ? nullptr : (T*)y.ptr;
+  signed char* qp = INT8 ? (signed char*)y.ptr : nullptr;
+#define LAUNCH()                                                            \
+  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;                            \
+  rms_fwd_kernel<T, VEC, TPR, NV, RES, INT8>                                \
+      <<<(unsigned)((rows + RPB - 1) / RPB), TPR < 256 ? 256 : TPR, 0,      \
+         lc.stream>>>(x.data<T>(), res.data<T>(), gamma.data<float>(), yp,  \
+                      qp, scale.data<float>(), sum.data<T>(),               \
+                      rstd.data<float>(), rows, C, eps)
+  RMS_DISPATCH((int)(16 / sizeof(T)))
+#undef LAUNCH
+  rms_fwd_long_kernel<T, RES, INT8>
+      <<<(unsigned)std::min<long>(rows, 4096), 1024, 0, lc.stream>>>(
+          x.data<T>(), res.data<T>(), gamma.data<float>(), yp, qp,
+          scale.data<float>(), sum.data<T>(), rstd.data<float>(), rows, C,
+          eps);
+}
+
+template <typename T, bool DSUM>
+void bwd_launch(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
+                const Arr& h, const Arr& gamma, const Arr& rstd,
+                const Arr& dx, float* partial, int nblk) {
+  const int C = (int)h.size(-1);
+  const long rows = h.numel() / C;
+  RowPlan p = plan_rows(rows, C, sizeof(T),
+                        aligned16({dy.ptr, dsum.ptr, h.ptr, gamma.ptr,
+                                   dx.ptr}));
+#define LAUNCH()                                                          \
+  rms_bwd_kernel<T, VEC, TPR, NV, DSUM>                                   \
+      <<<(unsigned)nblk, TPR < 256 ? 256 : TPR, 0, lc.stream>>>(          \
+          dy.data<T>(), dsum.data<T>(), h.data<T>(), gamma.data<float>(), \
+          rstd.data<float>(), dx.data<T>(), partial, rows, C)
+  RMS_DISPATCH((int)(16 / sizeof(T)))
+#undef LAUNCH
+  rms_bwd_long_kernel<T, DSUM>
+      <<<(unsigned)std::min<long>(rows, 4096), 1024, 0, lc.stream>>>(
+          dy.data<T>(), dsum.data<T>(), h.data<T>(), gamma.data<float>(),
+          rstd.data<float>(), dx.data<T>(), rows, C);
+  rms_dgamma_long_kernel<T>
+      <<<dim3((unsigned)((C + 255) / 256), (unsigned)nblk), 256, 0,
+         lc.stream>>>(dy.data<T>(), h.data<T>(), rstd.data<float>(), partial,
+                      rows, C);
+}
+
+}  // namespace
+
+void rms_norm_fwd_raw(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
+                      const Arr& residual, double eps, const Arr& y,
+                      const Arr& scale, const Arr& sum, const Arr& rstd) {
+  check_rows(x, gamma, "RMSNorm");
+  const bool res = residual.defined(), int8 = y.dtype == kInt8;
+  const long rows = x.numel() / x.size(-1);
+  if (rows == 0) return;
+  MX_CHECK(y.numel() == x.numel() && (int8 || y.dtype == x.dtype),
+           "RMSNorm: the output must have the data's size, and its type or "
+           "int8");
+  MX_CHECK(!res || (residual.numel() == x.numel() &&
+                    residual.dtype == x.dtype && sum.defined() &&
+                    sum.numel() == x.numel() && sum.dtype == x.dtype),
+           "RMSNorm: the residual and the sum must be like the data");
+  const Arr& stat = int8 ? scale : rstd;
+  MX_CHECK(stat.defined() && stat.dtype == kFloat32 && stat.numel() == rows,
+           "RMSNorm: one float32 value a row is needed beside the output");
+  DISPATCH_FLOAT_NATIVE(x.dtype, "RMSNorm", [&] {
+    auto go = [&](auto r, auto q) {
+      fwd_launch<scalar_t, decltype(r)::value, decltype(q)::value>(
+          lc, x, gamma, residual, eps, y, scale, sum, rstd);
+    };
+    if (res && int8) go(std::true_type{}, std::true_type{});
+    else if (res) go(std::true_type{}, std::false_type{});
+    else if (int8) go(std::false_type{}, std::true_type{});
+    else go(std::false_type{}, std::false_type{});
+  });
+  HIP_CHECK_LAST();
+}
+
+// two blocks for each of 256 CUs, and no more than there are rows for: the
+// partials are nblk rows to write and to read again
+int64_t rms_norm_bwd_blocks(int64_t rows) {
+  return std::max<int64_t>(1, std::min<int64_t>(rows, 512));
+}
+
+void rms_norm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
+                      const Arr& h, const Arr& gamma, const Arr& rstd,
+                      const Arr& dx, const Arr& dgamma, const Arr& partial) {
+  check_rows(h, gamma, "RMSNorm backward");
+  const int64_t C = h.size(-1), rows = h.numel() / C;
+  const int64_t nblk = rms_norm_bwd_blocks(rows);
+  MX_CHECK(dy.numel() == h.numel() && dy.dtype == h.dtype &&
+               dx.numel() == h.numel() && dx.dtype == h.dtype &&
+               (!dsum.defined() ||
+                (dsum.numel() == h.numel() && dsum.dtype == h.dtype)),
+           "RMSNorm backward: the gradients must be like the data");
+  MX_CHECK(rstd.dtype == kFloat32 && rstd.numel() == rows &&
+               dgamma.dtype == kFloat32 && dgamma.numel() == C &&
+               partial.dtype == kFloat32 && partial.numel() >= nblk * C,
+           "RMSNorm backward: statistics, dgamma or workspace too small");
+  DISPATCH_FLOAT_NATIVE(h.dtype, "RMSNorm backward", [&] {
+    if (rows == 0) return;
+    if (dsum.defined())
+      bwd_launch<scalar_t, true>(lc, dy, dsum, h, gamma, rstd, dx,
+                                 partial.data<float>(), (int)nblk);
+    else
+      bwd_launch<scalar_t, false>(lc, dy, dsum, h, gamma, rstd, dx,
+                                  partial.data<float>(), (int)nblk);
+  });
+  rms_dgamma_kernel<<<(unsigned)((C + 63) / 64), 1024, 0, lc.stream>>>(
+      partial.data<float>(), dgamma.data<float>(), rows ? (int)nblk : 0,
+      (int)C);
+  HIP_CHECK_LAST();
+}
+
+}  // namespace mxcore

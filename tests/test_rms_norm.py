@@ -1,0 +1,307 @@
+"""RMSNorm (with the residual's addition, and its int8 output) against the
+formula in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import mxnet_amd as mx
+from mxnet_amd import autograd
+from mxnet_amd.gluon import nn
+
+DEVICES = ['cpu', pytest.param('cuda:0', marks=pytest.mark.gpu)]
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+U32 = 2.0 ** -24  # half a step of float32
+
+
+def make(rows, cols, dtype, device, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    shape = (rows, cols)
+
+    def r(scale=1.0, dt=dtype, sh=shape):
+        return (torch.randn(*sh, generator=g) * scale).to(dt).to(device)
+
+    return dict(x=r(), res=r(2.0), gamma=1 + r(0.2, torch.float32, (cols,)),
+                dy=r(), dsum=r())
+
+
+def oracle(x, gamma, res=None, eps=1e-6):
+    h = x if res is None else (x.float() + res.float()).to(x.dtype)
+    v = h.double()
+    r = 1 / torch.sqrt(v.square().mean(-1, keepdim=True) + eps)
+    return h, r, v * r * gamma.double()
+
+
+def half_step(t):
+    # relative half step, and the absolute one of the smallest numbers
+    f = torch.finfo(t)
+    return f.eps / 2, f.smallest_normal * f.eps / 2
+
+
+def within(got, want, bound):
+    bad = (got.double() - want).abs() > bound
+    assert not bad.any(), (
+        int(bad.sum()), float(((got.double() - want).abs() - bound).max()))
+
+
+SHAPES = [(1, 1), (1, 8), (3, 7), (5, 64), (32, 1024), (2, 1001), (1, 4099),
+          (1500, 768), (1025, 2048), (3, 8192), (2, 20000), (1, 33000),
+          (1, 65544)]
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('with_res', [False, True])
+@pytest.mark.parametrize('rows,cols', SHAPES)
+def test_forward(rows, cols, with_res, dtype, device):
+    d = make(rows, cols, dtype, device)
+    res = d['res'] if with_res else None
+    out = mx.nd.RMSNorm(
+        mx.nd.from_torch(d['x']), mx.nd.from_torch(d['gamma']),
+        residual=mx.nd.from_torch(res) if with_res else None)
+    h, _, want = oracle(d['x'], d['gamma'], res)
+    if with_res:
+        out, total = out
+        assert torch.equal(total.to_torch(), h)
+    y = out.to_torch()
+    assert y.dtype == dtype and y.shape == d['x'].shape
+    # r is rounded once and there are two products: three half steps of
+    # float32 (four allow for their own products), then one of the type
+    rel, least = half_step(dtype)
+    within(y, want, want.abs() * (rel * (1 + 8 * U32) + 4 * U32) + least)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('with_res', [False, True])
+@pytest.mark.parametrize('rows,cols', [(1, 1), (3, 7), (5, 64), (700, 768),
+                                       (1030, 1000), (9, 1001), (3, 8192),
+                                       (2, 20000), (2, 65544)])
+def test_gradient(rows, cols, with_res, dtype, device):
+    d = make(rows, cols, dtype, device, seed=1)
+    x = mx.nd.from_torch(d['x'].clone().requires_grad_())
+    gamma = mx.nd.from_torch(d['gamma'].clone().requires_grad_())
+    dy, dsum = d['dy'].double(), d['dsum'].double()
+    with autograd.record():
+        if with_res:
+            res = mx.nd.from_torch(d['res'].clone().requires_grad_())
+            y, total = mx.nd.RMSNorm(x, gamma, residual=res)
+        else:
+            y = mx.nd.RMSNorm(x, gamma)
+    if with_res:
+        dx, dg, dres = (t.to_torch() for t in autograd.grad(
+            [y, total], [x, gamma, res],
+            [mx.nd.from_torch(d['dy']), mx.nd.from_torch(d['dsum'])]))
+        assert torch.equal(dx, dres)
+    else:
+        dx, dg = (t.to_torch() for t in autograd.grad(
+            [y], [x, gamma], [mx.nd.from_torch(d['dy'])]))
+        dsum = torch.zeros_like(dy)
+    h, r, _ = oracle(d['x'], d['gamma'], d['res'] if with_res else None)
+    g, n = dy * d['gamma'].double(), h.double() * r
+    m = (g * n).mean(-1, keepdim=True)
+    want = r * (g - n * m) + dsum
+    assert dx.dtype == dtype and dg.dtype == torch.float32
+    # a thread adds up to 64 products before six to ten levels of a tree; the
+    # terms are within that many half steps of float32, each of its own size.
+    # On the CPU autograd of the elementary operations rounds dy's path to
+    # the type where the norm was, and adds the sum's gradient in the type
+    rel, least = half_step(dtype)
+    terms = r * g.abs() + r * n.abs() * (
+        m.abs() + (g * n).abs().mean(-1, keepdim=True)) + dsum.abs()
+    steps = 1 if device != 'cpu' else 4
+    within(dx, want, terms * (100 * U32 + (steps - 1) * rel)
+           + want.abs() * rel * steps + steps * least)
+    # at most ceil(rows / blocks) + 32 + 16 additions in a row
+    within(dg, (dy * n).sum(0),
+           (dy * n).abs().sum(0) * U32 * (rows + 64) + 1e-30)
+
+
+def test_gradient_against_differences():
+    x = torch.randn(4, 9, dtype=torch.float32)
+    res, gamma = torch.randn(4, 9), torch.rand(9) + 0.5
+    dy, dsum = torch.randn(4, 9), torch.randn(4, 9)
+    xs = mx.nd.from_torch(x.clone().requires_grad_())
+    with autograd.record():
+        y, h = mx.nd.RMSNorm(xs, mx.nd.from_torch(gamma),
+                             residual=mx.nd.from_torch(res))
+    dx = autograd.grad([y, h], [xs], [mx.nd.from_torch(dy),
+                                      mx.nd.from_torch(dsum)])[0].to_torch()
+
+    def value(v):
+        s = v + res.double()
+        n = s / torch.sqrt(s.square().mean(-1, keepdim=True) + 1e-6)
+        return float((n * gamma.double() * dy).sum() + (s * dsum).sum())
+
+    step = 1e-5
+    for at in [(0, 0), (1, 4), (3, 8)]:
+        lo, hi = x.double(), x.double()
+        lo[at] -= step
+        hi[at] += step
+        # third derivatives are of the order of 1: the difference is off by
+        # about step^2, the gradient by a few half steps of float32
+        want = (value(hi) - value(lo)) / (2 * step)
+        assert abs(float(dx[at]) - want) < 1e-4
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('with_res', [False, True])
+@pytest.mark.parametrize('rows,cols', SHAPES)
+def test_int8(rows, cols, with_res, dtype, device):
+    d = make(rows, cols, dtype, device, seed=2)
+    d['x'][0] *= 30
+    res = d['res'] if with_res else None
+    out = mx.nd.RMSNorm(
+        mx.nd.from_torch(d['x']), mx.nd.from_torch(d['gamma']),
+        residual=mx.nd.from_torch(res) if with_res else None,
+        out_type='int8')
+    h, r, want = oracle(d['x'], d['gamma'], res)
+    q, scale = out[0].to_torch(), out[1].to_torch()
+    if with_res:
+        assert torch.equal(out[2].to_torch(), h)
+    assert q.dtype == torch.int8 and scale.shape == (rows, 1)
+    # the values, from r rounded to float32 once, are the definition's to the
+    # bit: every int8 is the one that the formula gives
+    y = h.float() * r.float() * d['gamma']
+    top = y.abs().amax(-1, keepdim=True)
+    assert torch.equal(scale, top * (1.0 / 127.0))
+    inv = torch.reciprocal(top) * 127.0
+    assert torch.equal(q, torch.round(y * inv).to(torch.int8))
+    # half a step of the scale, and what the factors and products round
+    within(q.double() * scale.double(), want,
+           scale.double() * (0.5 + 127 * 8 * U32))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('cols', [64, 1001, 33000])
+def test_int8_rows_without_scale(cols, device):
+    x = torch.randn(5, cols, device=device)
+    x[0] = 0
+    x[1, 3] = float('nan')
+    x[2, 4] = float('inf')
+    x[3, 5] = -float('inf')
+    q, scale = mx.nd.RMSNorm(mx.nd.from_torch(x),
+                             mx.nd.ones((cols,), ctx=mx.gpu(0) if device
+                                        != 'cpu' else mx.cpu()),
+                             out_type='int8')
+    q, scale = q.to_torch().cpu(), scale.to_torch().cpu()
+    assert not q[:4].any() and float(scale[0]) == 1.0
+    assert torch.isnan(scale[1:4]).all()
+    assert int(q[4].abs().max()) == 127 and float(scale[4]) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_views_on_the_gpu(dtype):
+    """Strided and misaligned inputs give what their copies give."""
+    big = torch.randn(40, 1030, device='cuda:0').to(dtype)
+    gamma = torch.rand(1024, device='cuda:0')
+    x, res = big[::2, 3:1027], big[1::2, 1:1025]
+    a = mx.nd.RMSNorm(mx.nd.from_torch(x), mx.nd.from_torch(gamma),
+                      residual=mx.nd.from_torch(res))
+    flat = torch.empty(20 * 1024 + 1, device='cuda:0', dtype=dtype)
+    odd = flat[1:].view(20, 1024)
+    odd.copy_(x)
+    b = mx.nd.RMSNorm(mx.nd.from_torch(odd), mx.nd.from_torch(gamma),
+                      residual=mx.nd.from_torch(res.contiguous()))
+    h, _, want = oracle(x, gamma, res)
+    rel, least = half_step(dtype)
+    for y, total in (a, b):
+        assert torch.equal(total.to_torch(), h)
+        within(y.to_torch(), want,
+               want.abs() * (rel * (1 + 8 * U32) + 4 * U32) + least)
+
+
+@pytest.mark.gpu
+def test_other_stream_and_graph():
+    d = make(64, 768, torch.float16, 'cuda:0', seed=3)
+    nd = mx.nd.from_torch
+    want = mx.nd.RMSNorm(nd(d['x']), nd(d['gamma']), residual=nd(d['res']))
+    want = [t.to_torch().clone() for t in want]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = mx.nd.RMSNorm(nd(d['x']), nd(d['gamma']), residual=nd(d['res']))
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a.to_torch(), b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        y, h = mx.nd.RMSNorm(nd(d['x']), nd(d['gamma']),
+                             residual=nd(d['res']))
+    for k in range(3):
+        d['x'].copy_(make(64, 768, torch.float16, 'cuda:0', seed=10 + k)['x'])
+        graph.replay()
+        torch.cuda.synchronize()
+        e = mx.nd.RMSNorm(nd(d['x']), nd(d['gamma']), residual=nd(d['res']))
+        assert torch.equal(y.to_torch(), e[0].to_torch())
+        assert torch.equal(h.to_torch(), e[1].to_torch())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_empty_and_unused(device):
+    x = torch.empty(0, 16, device=device, requires_grad=True)
+    gamma = torch.ones(16, device=device, requires_grad=True)
+    with autograd.record():
+        y = mx.nd.RMSNorm(mx.nd.from_torch(x), mx.nd.from_torch(gamma))
+    assert y.shape == (0, 16)
+    q, scale = mx.nd.RMSNorm(mx.nd.from_torch(x.detach()),
+                             mx.nd.from_torch(gamma.detach()),
+                             out_type='int8')
+    assert q.shape == (0, 16) and scale.shape == (0, 1)
+    # a loss of the sum alone
+    x = torch.randn(3, 16, device=device, requires_grad=True)
+    res = torch.randn(3, 16, device=device, requires_grad=True)
+    with autograd.record():
+        _, h = mx.nd.RMSNorm(mx.nd.from_torch(x), mx.nd.from_torch(gamma),
+                             residual=mx.nd.from_torch(res))
+        h.backward()
+    assert torch.equal(x.grad, torch.ones_like(x))
+    assert torch.equal(res.grad, torch.ones_like(x))
+
+
+def test_refusals():
+    nd = mx.nd.from_torch
+    x, gamma = torch.randn(2, 8), torch.ones(8)
+    with pytest.raises(TypeError):
+        mx.nd.RMSNorm(nd(x.double()), nd(gamma))
+    with pytest.raises(ValueError):
+        mx.nd.RMSNorm(nd(x), nd(torch.ones(7)))
+    with pytest.raises(ValueError):
+        mx.nd.RMSNorm(nd(x), nd(gamma), residual=nd(x[:1]))
+    with pytest.raises(ValueError):
+        mx.nd.RMSNorm(nd(x), nd(gamma), residual=nd(x.half()))
+    with pytest.raises(ValueError):
+        mx.nd.RMSNorm(nd(x), nd(gamma), out_type='uint8')
+    with pytest.raises(NotImplementedError):
+        mx.nd.RMSNorm(nd(x), nd(gamma), axis=0)
+    with pytest.raises(ValueError):
+        with autograd.record():
+            mx.nd.RMSNorm(nd(x.clone().requires_grad_()), nd(gamma),
+                          out_type='int8')
+
+
+def test_gluon_layer_and_symbol(tmp_path):
+    layer = nn.RMSNorm(epsilon=1e-5)
+    layer.initialize()
+    x, res = mx.nd.array(np.random.randn(3, 12)), \
+        mx.nd.array(np.random.randn(3, 12))
+    y = layer(x)
+    _, _, want = oracle(x.to_torch(), torch.ones(12), eps=1e-5)
+    within(y.to_torch(), want, want.abs() * 16 * U32)
+    y2, h = layer(x, res)
+    assert torch.equal(h.to_torch(), x.to_torch() + res.to_torch())
+    layer.cast('float16')
+    assert layer.gamma.data().dtype == np.float32
+    a, b, g = (mx.sym.var(n) for n in 'abg')
+    feed = {'a': x, 'b': res, 'g': mx.nd.ones((12,))}
+    ys, hs = mx.sym.RMSNorm(a, g, residual=b, eps=1e-5)
+    net = mx.sym.Group([ys, hs])
+    got = net.eval_dict(feed)
+    assert torch.equal(got[0].to_torch(), y2.to_torch())
+    assert torch.equal(got[1].to_torch(), h.to_torch())
+    net.save(str(tmp_path / 'n.json'))
+    got = mx.sym.load(str(tmp_path / 'n.json')).eval_dict(feed)
+    assert torch.equal(got[0].to_torch(), y2.to_torch())
+    assert torch.equal(mx.sym.RMSNorm(a, g, eps=1e-5).eval_dict(feed)[0]
+                       .to_torch(), y.to_torch())
