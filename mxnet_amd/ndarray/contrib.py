@@ -1,4 +1,6 @@
-"""Control-flow operators (reference src/operator/control_flow.cc:
+"""Contrib operators: attention over an encoder's states, and control flow.
+
+Control-flow operators (reference src/operator/control_flow.cc:
 ``_foreach``, ``_while_loop``, ``_cond`` and python wrappers
 python/mxnet/ndarray/contrib.py:foreach/while_loop/cond).
 
@@ -9,8 +11,10 @@ reference's stateful control-flow ops.
 import torch
 
 from .ndarray import NDArray
+from ..ops import contrib_transformer as _ct
 
-__all__ = ['foreach', 'while_loop', 'cond', 'isinf', 'isnan', 'isfinite']
+__all__ = ['foreach', 'while_loop', 'cond', 'isinf', 'isnan', 'isfinite',
+           'encdec_attention']
 
 
 def _as_list(x):
@@ -86,3 +90,25 @@ def isnan(data):
 
 def isfinite(data):
     return NDArray(torch.isfinite(data.handle))
+
+
+def encdec_attention(queries, keys_values, values=None, heads=1,
+                     kv_heads=None, valid_length=None, mask=None,
+                     layout='NTC'):
+    """Attention of a decoder's queries over an encoder's keys and values of
+    another length, in one kernel; differentiable in all of them.
+
+    queries (B, Sq, heads*D); keys_values (B, Sk, kv_heads*2*D) with each
+    head's key before its value (the layout of interleaved_matmul_encdec_qk),
+    or keys and ``values`` apart, (B, Sk, kv_heads*D) each; ``layout='TNC'``:
+    time first.  Consecutive query heads share a key head where kv_heads is
+    less than heads.  Keys from ``valid_length`` (B,) on and keys whose
+    ``mask`` (B, Sk) is 0 are left out, whatever their memory holds; a row
+    without a key gives zeros.  float16, bfloat16 and float32; head sizes up
+    to 128 on the GPU.
+    """
+    def t(x):
+        return None if x is None else x._t
+    return NDArray(_ct.encdec_attention(t(queries), t(keys_values), t(values),
+                                        heads, kv_heads, t(valid_length),
+                                        t(mask), layout))

@@ -194,6 +194,50 @@ def attention_bwd(dout, qkv, att, heads, temperature):
     return dqkv
 
 
+def _encdec_sizes(q, kv, heads, kv_heads, tnc):
+    sq, sk = q.shape[1], kv.shape[1]
+    B = q.shape[0]
+    if tnc:
+        B, sq, sk = q.shape[1], q.shape[0], kv.shape[0]
+    return B, heads, kv_heads, sq, sk, q.shape[2] // heads
+
+
+def _encdec_work(sizes, which, device):
+    n = _raw.encdec_attention_workspace(*sizes)[which]
+    return torch.empty((n,), dtype=torch.float32, device=device) if n else None
+
+
+def encdec_attention_fwd(q, kv, values, heads, kv_heads, length, mask, tnc,
+                         want_lse):
+    """(out, lse or None); lse is what the backward needs."""
+    q, kv = _c(q), _c(kv)
+    dev, s = _dev_stream(q)
+    sizes = _encdec_sizes(q, kv, heads, kv_heads, tnc)
+    out = torch.empty_like(q)
+    lse = torch.empty((sizes[0], heads, sizes[3]), dtype=torch.float32,
+                      device=q.device) if want_lse else None
+    work = _encdec_work(sizes, 0, q.device)
+    _raw.encdec_attention_fwd(dev, s, _arr(q), _arr(kv), _arr(values), heads,
+                              kv_heads, _arr(length), _arr(mask), tnc,
+                              _arr(out), _arr(lse), _arr(work))
+    return out, lse
+
+
+def encdec_attention_bwd(dout, q, kv, values, heads, kv_heads, length, mask,
+                         tnc, out, lse):
+    dout = _c(dout)
+    dev, s = _dev_stream(q)
+    sizes = _encdec_sizes(q, kv, heads, kv_heads, tnc)
+    dq, dkv = torch.empty_like(q), torch.empty_like(kv)
+    dvalues = torch.empty_like(values) if values is not None else None
+    work = _encdec_work(sizes, 1, q.device)
+    _raw.encdec_attention_bwd(dev, s, _arr(dout), _arr(q), _arr(kv),
+                              _arr(values), heads, kv_heads, _arr(length),
+                              _arr(mask), tnc, _arr(out), _arr(lse),
+                              _arr(dq), _arr(dkv), _arr(dvalues), _arr(work))
+    return dq, dkv, dvalues
+
+
 # ---------------------------------------------------------------------------
 # softmax / colsum
 # ---------------------------------------------------------------------------

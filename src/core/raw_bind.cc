@@ -196,6 +196,30 @@ void init_raw(py::module_& m) {
     rms_norm_bwd_raw(l.lc, ToArr(dy), ToArr(dsum), ToArr(h), ToArr(gamma),
                      ToArr(rstd), ToArr(dx), ToArr(dgamma), ToArr(partial));
   });
+  r.def("encdec_attention_workspace", &encdec_attention_workspace);
+  r.def("encdec_attention_fwd",
+        [](int dev, uintptr_t stream, py::handle q, py::handle kv,
+           py::handle values, int heads, int kv_heads, py::handle len,
+           py::handle mask, bool tnc, py::handle out, py::handle lse,
+           py::handle work) {
+          Launch l(dev, stream);
+          encdec_attention_fwd_raw(l.lc, ToArr(q), ToArr(kv), ToArr(values),
+                                   heads, kv_heads, ToArr(len), ToArr(mask),
+                                   tnc, ToArr(out), ToArr(lse), ToArr(work));
+        });
+  r.def("encdec_attention_bwd",
+        [](int dev, uintptr_t stream, py::handle dout, py::handle q,
+           py::handle kv, py::handle values, int heads, int kv_heads,
+           py::handle len, py::handle mask, bool tnc, py::handle out,
+           py::handle lse, py::handle dq, py::handle dkv, py::handle dvalues,
+           py::handle work) {
+          Launch l(dev, stream);
+          encdec_attention_bwd_raw(l.lc, ToArr(dout), ToArr(q), ToArr(kv),
+                                   ToArr(values), heads, kv_heads, ToArr(len),
+                                   ToArr(mask), tnc, ToArr(out), ToArr(lse),
+                                   ToArr(dq), ToArr(dkv), ToArr(dvalues),
+                                   ToArr(work));
+        });
   r.def("conv2d_fwd", [](int dev, uintptr_t stream, py::handle x,
                          py::handle w, py::handle bias, int sh, int sw,
                          int ph, int pw, int dh, int dw, int groups,

@@ -1,0 +1,1143 @@
+// Attention of a decoder over an encoder's states of another length.
+//
+//   S = Q K^T / sqrt(d),  P = softmax over the kept keys,  O = P V
+//   (a row without a key: zeros)
+//   dV = P^T dO,  dP = dO V^T,  D = sum_d dO * O,  dS = P * (dP - D)
+//   dQ = dS K / sqrt(d),  dK = dS^T Q / sqrt(d)
+//
+// The scores are never stored: one pass over the keys with the running
+// maximum and sum of the softmax, and the backward computes P again from the
+// row's log-sum, which the forward stores.  Query heads that share a key head
+// are rows of one matrix (row m = g * Sq + s for the g-th of them), so shared
+// keys are read once and their gradient is summed in the accumulators.
+//
+// Products run on the matrix cores with 32-bit accumulators, 32x32 tiles:
+// lane l (h = l / 32) holds of A row l % 32 and of B column l % 32, elements
+// k = 8 h + j; of C column l % 32, and in register i row
+// 8 (i / 4) + 4 h + i % 4.  The forward computes S transposed (keys by
+// queries): a query's scores lie in one lane pair's registers, the softmax
+// needs one exchange between the two, and the registers ARE the B operand of
+// the next product when its 16 keys are taken in the order
+// {4h..4h+3, 8+4h..8+4h+3}; V's fragment is read in that order by the
+// transposing LDS load.  dQ does the same with dS; dK and dV use S untransposed,
+// whose registers are the A operand of P^T dO and dS^T Q.
+//
+// fp32 uses the fp32 matrix instructions (eight of k = 2 for one of k = 16).
+#include "ops_api.h"
+
+namespace mxcore {
+namespace {
+
+typedef short trs4_t __attribute__((ext_vector_type(4)));
+typedef float float8_t __attribute__((ext_vector_type(8)));
+
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T> struct Mat;
+template <> struct Mat<_Float16> {
+  using Frag = half8_t;
+  static DEV_INLINE float16_t mma(Frag a, Frag b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Mat<__bf16> {
+  using Frag = bf168_t;
+  static DEV_INLINE float16_t mma(Frag a, Frag b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Mat<float> {
+  using Frag = float8_t;
+  static DEV_INLINE float16_t mma(Frag a, Frag b, float16_t c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// one [B, S, heads, D] view: strides in elements, D contiguous
+struct View {
+  void* p;
+  long sb, ss, sh;
+};
+
+struct Att {
+  View q, k, v, o, dout, dq, dk, dv;
+  const int* len;        // [B] or null
+  const uint8_t* mask;   // [B, Sk], 0: masked, or null
+  float* lse;            // [B, H, Sq] log2 of the row's sum, +inf: no key
+  float* delta;          // [B, H, Sq]
+  float* part;           // partial results of a split, fp32
+  int B, H, Hk, G, Sq, Sk, D;
+  int nsplit;
+  int vec;               // 16-byte accesses
+  float scale;           // 1 / sqrt(D)
+};
+
+// ---------------------------------------------------------------------------
+// LDS tiles [rows][DP] in 16-byte chunks.  The chunk's place in its row is
+// XORed with a function of the row, chosen so that both readers are free of
+// bank conflicts: 16 rows at one chunk (row fragments), and 4 rows at 4
+// neighbouring chunks (the transposing read).
+// ---------------------------------------------------------------------------
+template <typename T, int DP>
+struct Tile {
+  static constexpr int EPC = 16 / sizeof(T);  // elements a chunk
+  static constexpr int CPR = DP / EPC;        // chunks a row
+  static constexpr int RB = DP * (int)sizeof(T);
+  static DEV_INLINE int swz(int row) {
+    if constexpr (RB == 64) return (row >> 2) & 3;
+    if constexpr (RB == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    return ((row & 3) << 2) | ((row >> 2) & 3);
+  }
+  // byte offset of a chunk
+  static DEV_INLINE int at(int row, int chunk) {
+    return row * RB + ((chunk ^ swz(row)) << 4);
+  }
+  // elements d = 16 ks + 8 h + j of one row
+  static DEV_INLINE typename Mat<T>::Frag row_frag(const char* t, int row,
+                                                   int ks, int h) {
+    typename Mat<T>::Frag f;
+    if constexpr (sizeof(T) == 2) {
+      f = *(const typename Mat<T>::Frag*)(t + at(row, ks * 2 + h));
+    } else {
+      const float4_t a = *(const float4_t*)(t + at(row, ks * 4 + h * 2));
+      const float4_t b = *(const float4_t*)(t + at(row, ks * 4 + h * 2 + 1));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[j] = a[j];
+        f[4 + j] = b[j];
+      }
+    }
+    return f;
+  }
+  // column c0 + l % 32, rows k0 + {4h..4h+3, 8+4h..8+4h+3}
+  static DEV_INLINE typename Mat<T>::Frag col_frag(const char* t, int k0,
+                                                   int c0, int l) {
+    typename Mat<T>::Frag f;
+    const int h = l >> 5;
+    if constexpr (sizeof(T) == 2) {
+      // 16 lanes read four rows of 16 columns and get one column each
+      const int row = k0 + 4 * h + ((l & 15) >> 2);
+      const int col = c0 + ((l >> 4) & 1) * 16 + (l & 3) * 4;
+      const int sub = (col & 4) * 2;  // which half of the chunk, in bytes
+      union {
+        trs4_t s[2];
+        typename Mat<T>::Frag f;
+      } u;
+      u.s[0] = tr(t + at(row, col >> 3) + sub);
+      u.s[1] = tr(t + at(row + 8, col >> 3) + sub);
+      f = u.f;
+    } else {
+      const int col = c0 + (l & 31);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = k0 + 4 * h + (j & 3) + (j >> 2) * 8;
+        f[j] = *(const float*)(t + at(row, col >> 2) + (col & 3) * 4);
+      }
+    }
+    return f;
+  }
+  static DEV_INLINE trs4_t tr(const char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) trs4_t*)(uintptr_t)p);
+  }
+};
+
+// 16 bytes of a row from element d on; zeros from D on
+template <typename T>
+DEV_INLINE int4_t load_chunk(const T* row, int d, int D, bool vec) {
+  int4_t r = {0, 0, 0, 0};
+  if (vec) {
+    if (d < D) r = *(const int4_t*)(row + d);
+  } else {
+    constexpr int N = 16 / sizeof(T);
+    union {
+      T e[N];
+      int4_t v;
+    } u;
+    u.v = r;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (d + j < D) u.e[j] = row[d + j];
+    r = u.v;
+  }
+  return r;
+}
+
+// fragment elements d = 16 ks + 8 h + j straight from a row in memory
+template <typename T>
+DEV_INLINE typename Mat<T>::Frag load_frag(const T* row, int ks, int h, int D,
+                                           bool vec, bool valid) {
+  union {
+    int4_t c[sizeof(T) / 2];
+    typename Mat<T>::Frag f;
+  } u;
+  constexpr int N = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+    u.c[i] = int4_t{0, 0, 0, 0};
+    if (valid) u.c[i] = load_chunk<T>(row, ks * 16 + h * 8 + i * N, D, vec);
+  }
+  return u.f;
+}
+
+// the fragment of accumulator registers r0..r0+7, rounded to the type
+template <typename T>
+DEV_INLINE typename Mat<T>::Frag pack(const float16_t& a, int r0) {
+  typename Mat<T>::Frag f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)a[r0 + j];
+  return f;
+}
+
+template <typename T>
+DEV_INLINE const T* row_ptr(const View& v, long b, int head, int s) {
+  return (const T*)v.p + b * v.sb + s * v.ss + head * v.sh;
+}
+
+// row m of the G * Sq rows that share a key head
+template <typename T>
+DEV_INLINE T* q_row(const View& v, const Att& a, long b, int hk, int m) {
+  const int g = m / a.Sq;
+  return (T*)row_ptr<T>(v, b, hk * a.G + g, m - g * a.Sq);
+}
+
+DEV_INLINE int kept_keys(const Att& a, int b) {
+  int n = a.Sk;
+  if (a.len) n = min(n, max(0, a.len[b]));
+  return n;
+}
+
+// ---------------------------------------------------------------------------
+// staging: NT threads bring ROWS rows of DP elements to registers, then LDS.
+// A key that is masked or past the length is stored as zeros, whatever its
+// memory holds, so that a NaN there meets no product.
+// ---------------------------------------------------------------------------
+template <typename T, int DP, int ROWS, int NT>
+struct Stage {
+  using TL = Tile<T, DP>;
+  static constexpr int N = (ROWS * TL::CPR + NT - 1) / NT;
+  int4_t r[N];
+  // row(i) gives the i-th row's address or null
+  template <typename F>
+  DEV_INLINE void load(F row, int t, int D, bool vec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = i * NT + t;
+      r[i] = int4_t{0, 0, 0, 0};
+      if ((ROWS * TL::CPR) % NT == 0 || c < ROWS * TL::CPR) {
+        const T* p = row(c / TL::CPR);
+        if (p) r[i] = load_chunk<T>(p, (c % TL::CPR) * TL::EPC, D, vec);
+      }
+    }
+  }
+  DEV_INLINE void store(char* tile, int t) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = i * NT + t;
+      if ((ROWS * TL::CPR) % NT == 0 || c < ROWS * TL::CPR)
+        *(int4_t*)(tile + TL::at(c / TL::CPR, c % TL::CPR)) = r[i];
+    }
+  }
+};
+
+// O^T (or dQ^T) accumulators of one row per lane pair to memory
+template <typename T, int DP>
+DEV_INLINE void store_row(T* row, const float16_t (&acc)[DP / 32], float f,
+                          int h, int D, bool vec) {
+  using V4 = T __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = n * 32 + 2 * i + 4 * h;
+      if (vec) {
+        if (d < D) {
+          V4 o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = (T)(acc[n][i + j] * f);
+          *(V4*)(row + d) = o;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d + j < D) row[d + j] = (T)(acc[n][i + j] * f);
+      }
+    }
+}
+
+template <int DP>
+DEV_INLINE void store_part(float* row, const float16_t (&acc)[DP / 32],
+                           int h) {
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      float4_t o = {acc[n][i], acc[n][i + 1], acc[n][i + 2], acc[n][i + 3]};
+      *(float4_t*)(row + n * 32 + 2 * i + 4 * h) = o;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// one tile's step of the running softmax: KB blocks of 32 keys in `s`
+// (transposed scores, raw), O^T in `acc`; m and l are the row's reference
+// maximum (raw) and this lane's share of the sum.
+// ---------------------------------------------------------------------------
+template <typename T, int DP, int KB>
+DEV_INLINE void softmax_step(float16_t (&s)[KB], float16_t (&acc)[DP / 32],
+                             float& m, float& l, float c) {
+  float top = kNegInf;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  // The reference follows the maximum only when that leaves it by more than
+  // 2^8: until then the weights are at most 256, which no accumulator
+  // minds, and the output is not scaled again
+  const bool move = (top - m) * c > 8.f || (m == kNegInf && top > m);
+  if (__any(move)) {
+    const float to = move ? top : m;
+    const float f = to == kNegInf ? 1.f
+                                  : __builtin_amdgcn_exp2f((m - to) * c);
+    m = to;
+    l *= f;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[n][i] *= f;
+  }
+  const float off = m == kNegInf ? 0.f : m * c;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -off));
+      l += s[kb][i];
+    }
+}
+
+// scores of KB blocks of 32 keys, transposed
+template <typename T, int DP, int KB>
+DEV_INLINE void scores(const char* kt,
+                       const typename Mat<T>::Frag (&qf)[DP / 16],
+                       float16_t (&s)[KB], int l) {
+  const int r = l & 31, h = l >> 5;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    s[kb] = float16_t{};
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks)
+      s[kb] = Mat<T>::mma(Tile<T, DP>::row_frag(kt, kb * 32 + r, ks, h),
+                          qf[ks], s[kb]);
+  }
+}
+
+// acc += (tile's columns) x (weights): O^T += V^T P^T, dQ^T += K^T dS^T
+template <typename T, int DP, int KB>
+DEV_INLINE void weigh(const char* t, const float16_t (&s)[KB],
+                      float16_t (&acc)[DP / 32], int l) {
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const auto p = pack<T>(s[kb], k * 8);
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n)
+        acc[n] = Mat<T>::mma(
+            Tile<T, DP>::col_frag(t, kb * 32 + k * 16, n * 32, l), p, acc[n]);
+    }
+}
+
+// keys that are not kept get a score of -inf; `keep` holds a byte a key
+template <int KB>
+DEV_INLINE void drop_keys(const uint8_t* keep, float16_t (&s)[KB], int h) {
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const uint32_t k4 = *(const uint32_t*)(keep + kb * 32 + 2 * i + 4 * h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!((k4 >> (8 * j)) & 0xff)) s[kb][i + j] = kNegInf;
+    }
+}
+
+// the workspace of a split: [split][B * Hk][rows][DP] values, then for the
+// forward [split][B * Hk][rows][2] maxima and sums
+DEV_INLINE long part_row(const Att& a, int split, long bh, int m) {
+  return ((long)split * a.B * a.Hk + bh) * (a.G * (long)a.Sq) + m;
+}
+
+template <typename T, int DP>
+DEV_INLINE void finish_row(const Att& a, const float16_t (&acc)[DP / 32],
+                           float m, float l, int split, int b, int hk,
+                           int row, int h) {
+  const int M = a.G * a.Sq;
+  if (row >= M) return;
+  const float c = a.scale * kLog2e;
+  const long bh = (long)b * a.Hk + hk;
+  if (a.nsplit > 1) {
+    const long at = part_row(a, split, bh, row);
+    store_part<DP>(a.part + at * DP, acc, h);
+    if (h == 0) {
+      float* ml = a.part + (long)a.nsplit * a.B * a.Hk * M * DP + at * 2;
+      ml[0] = m;
+      ml[1] = l;
+    }
+    return;
+  }
+  store_row<T, DP>(q_row<T>(a.o, a, b, hk, row), acc, l > 0.f ? 1.f / l : 0.f,
+                   h, a.D, a.vec);
+  if (a.lse && h == 0)
+    a.lse[bh * M + row] = l > 0.f ? m * c + __builtin_amdgcn_logf(l)
+                                  : -kNegInf;
+}
+
+// ---------------------------------------------------------------------------
+// forward: NW waves of 32 rows each over tiles of BN keys that all share
+// ---------------------------------------------------------------------------
+template <typename T, int DP, int NW, int BN>
+__global__ __launch_bounds__(NW * 64) void att_fwd_kernel(Att a) {
+  using TL = Tile<T, DP>;
+  constexpr int NT = NW * 64, KB = BN / 32, BYTES = BN * TL::RB;
+  __shared__ __attribute__((aligned(16))) char lk[2][BYTES], lv[2][BYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t lkeep[2][BN];
+  const int M = a.G * a.Sq, mt = (M + NW * 32 - 1) / (NW * 32);
+  int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int tile = id % mt;
+  id /= mt;
+  const int split = id % a.nsplit;
+  const int bh = id / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int t = threadIdx.x, l = t & 63, h = l >> 5;
+  const int row = tile * NW * 32 + (t >> 6) * 32 + (l & 31);
+  const bool vec = a.vec;
+  const int n = kept_keys(a, b);
+  const int tiles = (n + BN - 1) / BN;
+  const int t0 = (int)((long)tiles * split / a.nsplit);
+  const int t1 = (int)((long)tiles * (split + 1) / a.nsplit);
+  const uint8_t* mask = a.mask ? a.mask + (long)b * a.Sk : nullptr;
+
+  typename Mat<T>::Frag qf[DP / 16];
+  const T* qr = row < M ? q_row<T>(a.q, a, b, hk, row) : nullptr;
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks)
+    qf[ks] = load_frag<T>(qr, ks, h, a.D, vec, row < M);
+  float16_t acc[DP / 32] = {};
+  float m = kNegInf, sum = 0.f;
+
+  Stage<T, DP, BN, NT> sk, sv;
+  auto keep = [&](int key) {
+    return key < n && (!mask || mask[key]);
+  };
+  auto fetch = [&](int i) {
+    sk.load([&](int r) {
+      const int key = i * BN + r;
+      return keep(key) ? row_ptr<T>(a.k, b, hk, key) : nullptr;
+    }, t, a.D, vec);
+    sv.load([&](int r) {
+      const int key = i * BN + r;
+      return keep(key) ? row_ptr<T>(a.v, b, hk, key) : nullptr;
+    }, t, a.D, vec);
+  };
+  auto put = [&](int i, int buf) {
+    sk.store(lk[buf], t);
+    sv.store(lv[buf], t);
+    for (int r = t; r < BN; r += NT) lkeep[buf][r] = keep(i * BN + r);
+  };
+  if (t0 < t1) {
+    fetch(t0);
+    put(t0, 0);
+  }
+  __syncthreads();
+  for (int i = t0; i < t1; ++i) {
+    const int buf = (i - t0) & 1;
+    if (i + 1 < t1) fetch(i + 1);
+    float16_t s[KB];
+    scores<T, DP, KB>(lk[buf], qf, s, l);
+    if (mask || (i + 1) * BN > n) drop_keys<KB>(lkeep[buf], s, h);
+    softmax_step<T, DP, KB>(s, acc, m, sum, a.scale * kLog2e);
+    weigh<T, DP, KB>(lv[buf], s, acc, l);
+    if (i + 1 < t1) put(i + 1, buf ^ 1);
+    __syncthreads();
+  }
+  sum += __shfl_xor(sum, 32, 64);
+  finish_row<T, DP>(a, acc, m, sum, split, b, hk, row, h);
+}
+
+// ---------------------------------------------------------------------------
+// forward of at most 32 rows (single tokens): each of 4 waves takes its own
+// keys, in its own part of LDS and without a barrier; the waves' results are
+// joined at the end.
+// ---------------------------------------------------------------------------
+template <typename T, int DP, int BN>
+__global__ __launch_bounds__(256) void att_token_kernel(Att a) {
+  using TL = Tile<T, DP>;
+  constexpr int NW = 4, KB = BN / 32, BYTES = BN * TL::RB;
+  constexpr int JOIN = 32 * (DP + 4) * 4;  // one wave's O^T, m and l
+  constexpr int PER_WAVE = 2 * BYTES > JOIN ? 2 * BYTES : JOIN;
+  __shared__ __attribute__((aligned(16))) char lds[NW][PER_WAVE];
+  __shared__ __attribute__((aligned(16))) uint8_t lkeep[NW][BN];
+  const int M = a.G * a.Sq;
+  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int split = id % a.nsplit;
+  const int bh = id / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int t = threadIdx.x, l = t & 63, h = l >> 5, w = t >> 6;
+  const int row = l & 31;
+  const bool vec = a.vec;
+  const int n = kept_keys(a, b);
+  const int tiles = (n + BN - 1) / BN, parts = a.nsplit * NW;
+  const int t0 = (int)((long)tiles * (split * NW + w) / parts);
+  const int t1 = (int)((long)tiles * (split * NW + w + 1) / parts);
+  const uint8_t* mask = a.mask ? a.mask + (long)b * a.Sk : nullptr;
+
+  typename Mat<T>::Frag qf[DP / 16];
+  const T* qr = row < M ? q_row<T>(a.q, a, b, hk, row) : nullptr;
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks)
+    qf[ks] = load_frag<T>(qr, ks, h, a.D, vec, row < M);
+  float16_t acc[DP / 32] = {};
+  float m = kNegInf, sum = 0.f;
+  char *lk = lds[w], *lv = lds[w] + BYTES;
+
+  Stage<T, DP, BN, 64> sk, sv;
+  auto keep = [&](int key) {
+    return key < n && (!mask || mask[key]);
+  };
+  auto fetch = [&](int i) {
+    sk.load([&](int r) {
+      const int key = i * BN + r;
+      return keep(key) ? row_ptr<T>(a.k, b, hk, key) : nullptr;
+    }, l, a.D, vec);
+    sv.load([&](int r) {
+      const int key = i * BN + r;
+      return keep(key) ? row_ptr<T>(a.v, b, hk, key) : nullptr;
+    }, l, a.D, vec);
+  };
+  if (t0 < t1) fetch(t0);
+  for (int i = t0; i < t1; ++i) {
+    sk.store(lk, l);
+    sv.store(lv, l);
+    if (l < BN) lkeep[w][l] = keep(i * BN + l);
+    // a wave's LDS accesses are done in order; the fence keeps the compiler
+    // from moving the reads of other lanes' values over these writes
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (i + 1 < t1) fetch(i + 1);
+    float16_t s[KB];
+    scores<T, DP, KB>(lk, qf, s, l);
+    if (mask || (i + 1) * BN > n) drop_keys<KB>(lkeep[w], s, h);
+    softmax_step<T, DP, KB>(s, acc, m, sum, a.scale * kLog2e);
+    weigh<T, DP, KB>(lv, s, acc, l);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  sum += __shfl_xor(sum, 32, 64);
+
+  // join the waves: O^T as rows of DP + 4 values (the pad keeps the 32 rows
+  // off each other's banks), then m and l behind them
+  __syncthreads();
+  float* mine = (float*)lds[w] + row * (DP + 4);
+  store_part<DP>(mine, acc, h);
+  if (h == 0) {
+    mine[DP] = m;
+    mine[DP + 1] = sum;
+  }
+  __syncthreads();
+  if (w != 0) return;
+  float top = kNegInf;
+  const float c = a.scale * kLog2e;
+#pragma unroll
+  for (int k = 0; k < NW; ++k)
+    top = fmaxf(top, ((const float*)lds[k])[row * (DP + 4) + DP]);
+  sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < DP / 32; ++k) acc[k] = float16_t{};
+#pragma unroll
+  for (int k = 0; k < NW; ++k) {
+    const float* o = (const float*)lds[k] + row * (DP + 4);
+    const float f = o[DP] == kNegInf
+                        ? 0.f : __builtin_amdgcn_exp2f((o[DP] - top) * c);
+    sum += o[DP + 1] * f;
+#pragma unroll
+    for (int nn = 0; nn < DP / 32; ++nn)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const float4_t v = *(const float4_t*)(o + nn * 32 + 2 * i + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[nn][i + j] += v[j] * f;
+      }
+  }
+  finish_row<T, DP>(a, acc, top, sum, split, b, hk, row, h);
+}
+
+// joins the splits of the forward: a wave a row
+template <typename T>
+__global__ __launch_bounds__(256) void att_join_kernel(Att a, int DP) {
+  const int M = a.G * a.Sq, l = threadIdx.x & 63;
+  const long rows = (long)a.B * a.Hk * M;
+  const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  const float* ml = a.part + (long)a.nsplit * rows * DP;
+  const float c = a.scale * kLog2e;
+  float top = kNegInf;
+  for (int k = 0; k < a.nsplit; ++k)
+    top = fmaxf(top, ml[(k * rows + at) * 2]);
+  float sum = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int k = 0; k < a.nsplit; ++k) {
+    const float m = ml[(k * rows + at) * 2];
+    if (m == kNegInf) continue;
+    const float f = __builtin_amdgcn_exp2f((m - top) * c);
+    const float* o = a.part + (k * rows + at) * DP;
+    sum += ml[(k * rows + at) * 2 + 1] * f;
+    if (l < DP) o0 += o[l] * f;
+    if (l + 64 < DP) o1 += o[l + 64] * f;
+  }
+  const long bh = at / M;
+  const int m = (int)(at - bh * M);
+  T* out = q_row<T>(a.o, a, bh / a.Hk, (int)(bh % a.Hk), m);
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  if (l < a.D) out[l] = (T)(o0 * inv);
+  if (l + 64 < a.D) out[l + 64] = (T)(o1 * inv);
+  if (a.lse && l == 0)
+    a.lse[at] = sum > 0.f ? top * c + __builtin_amdgcn_logf(sum) : -kNegInf;
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+// delta = sum_d dO * O: a wave a row
+template <typename T>
+__global__ __launch_bounds__(256) void att_delta_kernel(Att a) {
+  const int M = a.G * a.Sq, l = threadIdx.x & 63;
+  const long rows = (long)a.B * a.Hk * M;
+  const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  const long bh = at / M;
+  const int m = (int)(at - bh * M), b = (int)(bh / a.Hk),
+            hk = (int)(bh % a.Hk);
+  const T* o = q_row<T>(a.o, a, b, hk, m);
+  const T* g = q_row<T>(a.dout, a, b, hk, m);
+  float v = 0.f;
+  for (int d = l; d < a.D; d += 64) v += (float)o[d] * (float)g[d];
+  v = wave_reduce_sum(v);
+  if (l == 0) a.delta[at] = v;
+}
+
+// dQ: rows as in the forward, over all keys (or a split's)
+template <typename T, int DP, int NW, int BN>
+__global__ __launch_bounds__(NW * 64) void att_dq_kernel(Att a) {
+  using TL = Tile<T, DP>;
+  constexpr int NT = NW * 64, KB = BN / 32, BYTES = BN * TL::RB;
+  __shared__ __attribute__((aligned(16))) char lk[2][BYTES], lv[2][BYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t lkeep[2][BN];
+  const int M = a.G * a.Sq, mt = (M + NW * 32 - 1) / (NW * 32);
+  int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int tile = id % mt;
+  id /= mt;
+  const int split = id % a.nsplit;
+  const int bh = id / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int t = threadIdx.x, l = t & 63, h = l >> 5, r = l & 31;
+  const int row = tile * NW * 32 + (t >> 6) * 32 + r;
+  const bool vec = a.vec;
+  const int n = kept_keys(a, b);
+  const int tiles = (n + BN - 1) / BN;
+  const int t0 = (int)((long)tiles * split / a.nsplit);
+  const int t1 = (int)((long)tiles * (split + 1) / a.nsplit);
+  const uint8_t* mask = a.mask ? a.mask + (long)b * a.Sk : nullptr;
+  const float c = a.scale * kLog2e;
+
+  typename Mat<T>::Frag qf[DP / 16], gf[DP / 16];
+  const T* qr = row < M ? q_row<T>(a.q, a, b, hk, row) : nullptr;
+  const T* gr = row < M ? q_row<T>(a.dout, a, b, hk, row) : nullptr;
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    qf[ks] = load_frag<T>(qr, ks, h, a.D, vec, row < M);
+    gf[ks] = load_frag<T>(gr, ks, h, a.D, vec, row < M);
+  }
+  const float lse = row < M ? a.lse[(long)bh * M + row] : -kNegInf;
+  const float delta = row < M ? a.delta[(long)bh * M + row] : 0.f;
+  float16_t acc[DP / 32] = {};
+
+  Stage<T, DP, BN, NT> sk, sv;
+  auto keep = [&](int key) {
+    return key < n && (!mask || mask[key]);
+  };
+  auto fetch = [&](int i) {
+    sk.load([&](int rr) {
+      const int key = i * BN + rr;
+      return keep(key) ? row_ptr<T>(a.k, b, hk, key) : nullptr;
+    }, t, a.D, vec);
+    sv.load([&](int rr) {
+      const int key = i * BN + rr;
+      return keep(key) ? row_ptr<T>(a.v, b, hk, key) : nullptr;
+    }, t, a.D, vec);
+  };
+  auto put = [&](int i, int buf) {
+    sk.store(lk[buf], t);
+    sv.store(lv[buf], t);
+    for (int k = t; k < BN; k += NT) lkeep[buf][k] = keep(i * BN + k);
+  };
+  if (t0 < t1) {
+    fetch(t0);
+    put(t0, 0);
+  }
+  __syncthreads();
+  for (int i = t0; i < t1; ++i) {
+    const int buf = (i - t0) & 1;
+    if (i + 1 < t1) fetch(i + 1);
+    float16_t s[KB], dp[KB];
+    scores<T, DP, KB>(lk[buf], qf, s, l);
+    scores<T, DP, KB>(lv[buf], gf, dp, l);
+    if (mask || (i + 1) * BN > n) drop_keys<KB>(lkeep[buf], s, h);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        s[kb][j] = __builtin_amdgcn_exp2f(fmaf(s[kb][j], c, -lse)) *
+                   (dp[kb][j] - delta);
+    weigh<T, DP, KB>(lk[buf], s, acc, l);
+    if (i + 1 < t1) put(i + 1, buf ^ 1);
+    __syncthreads();
+  }
+  if (row >= M) return;
+  if (a.nsplit > 1)
+    store_part<DP>(a.part + part_row(a, split, bh, row) * DP, acc, h);
+  else
+    store_row<T, DP>(q_row<T>(a.dq, a, b, hk, row), acc, a.scale, h, a.D,
+                     vec);
+}
+
+// dK and dV: NW waves of 32 keys each over tiles of BM rows (or a split's)
+template <typename T, int DP, int NW, int BM>
+__global__ __launch_bounds__(NW * 64) void att_dkv_kernel(Att a) {
+  using TL = Tile<T, DP>;
+  constexpr int NT = NW * 64, BYTES = BM * TL::RB;
+  __shared__ __attribute__((aligned(16))) char lq[2][BYTES], lg[2][BYTES];
+  __shared__ __attribute__((aligned(16))) float llse[2][BM], ldel[2][BM];
+  const int M = a.G * a.Sq, kt = (a.Sk + NW * 32 - 1) / (NW * 32);
+  int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int tile = id % kt;
+  id /= kt;
+  const int split = id % a.nsplit;
+  const int bh = id / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int t = threadIdx.x, l = t & 63, h = l >> 5, r = l & 31;
+  const int k0 = tile * NW * 32 + (t >> 6) * 32, key = k0 + r;
+  const bool vec = a.vec;
+  const int n = kept_keys(a, b);
+  const bool keep = key < n && (!a.mask || a.mask[(long)b * a.Sk + key]);
+  const float c = a.scale * kLog2e;
+  // a block whose keys are all past the length only writes its zeros
+  const int tiles = tile * NW * 32 < n ? (M + BM - 1) / BM : 0;
+  const int t0 = (int)((long)tiles * split / a.nsplit);
+  const int t1 = (int)((long)tiles * (split + 1) / a.nsplit);
+
+  typename Mat<T>::Frag kf[DP / 16], vf[DP / 16];
+  const T* kr = keep ? row_ptr<T>(a.k, b, hk, key) : nullptr;
+  const T* vr = keep ? row_ptr<T>(a.v, b, hk, key) : nullptr;
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    kf[ks] = load_frag<T>(kr, ks, h, a.D, vec, keep);
+    vf[ks] = load_frag<T>(vr, ks, h, a.D, vec, keep);
+  }
+  float16_t dk[DP / 32] = {}, dv[DP / 32] = {};
+
+  Stage<T, DP, BM, NT> sq, sg;
+  auto fetch = [&](int i) {
+    sq.load([&](int rr) -> const T* {
+      const int m = i * BM + rr;
+      return m < M ? q_row<T>(a.q, a, b, hk, m) : nullptr;
+    }, t, a.D, vec);
+    sg.load([&](int rr) -> const T* {
+      const int m = i * BM + rr;
+      return m < M ? q_row<T>(a.dout, a, b, hk, m) : nullptr;
+    }, t, a.D, vec);
+  };
+  auto put = [&](int i, int buf) {
+    sq.store(lq[buf], t);
+    sg.store(lg[buf], t);
+    for (int k = t; k < BM; k += NT) {
+      const int m = i * BM + k;
+      // a row past the end has a weight of exp2(-inf)
+      llse[buf][k] = m < M ? a.lse[(long)bh * M + m] : -kNegInf;
+      ldel[buf][k] = m < M ? a.delta[(long)bh * M + m] : 0.f;
+    }
+  };
+  if (t0 < t1) {
+    fetch(t0);
+    put(t0, 0);
+  }
+  __syncthreads();
+  for (int i = t0; i < t1; ++i) {
+    const int buf = (i - t0) & 1;
+    if (i + 1 < t1) fetch(i + 1);
+#pragma unroll
+    for (int mb = 0; mb < BM / 32; ++mb) {
+      float16_t s = {}, dp = {};
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks)
+        s = Mat<T>::mma(TL::row_frag(lq[buf], mb * 32 + r, ks, h), kf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks)
+        dp = Mat<T>::mma(TL::row_frag(lg[buf], mb * 32 + r, ks, h), vf[ks],
+                         dp);
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const int at = mb * 32 + 2 * j + 4 * h;
+        const float4_t lse = *(const float4_t*)&llse[buf][at];
+        const float4_t del = *(const float4_t*)&ldel[buf][at];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[j + e], c, -lse[e]));
+          p = keep ? p : 0.f;
+          s[j + e] = p;
+          dp[j + e] = p * (dp[j + e] - del[e]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const auto p = pack<T>(s, k * 8), ds = pack<T>(dp, k * 8);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          dv[d] = Mat<T>::mma(
+              p, TL::col_frag(lg[buf], mb * 32 + k * 16, d * 32, l), dv[d]);
+          dk[d] = Mat<T>::mma(
+              ds, TL::col_frag(lq[buf], mb * 32 + k * 16, d * 32, l), dk[d]);
+        }
+      }
+    }
+    if (i + 1 < t1) put(i + 1, buf ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int k = k0 + 8 * (j / 4) + 4 * h + (j & 3), col = d * 32 + r;
+      if (k >= a.Sk) continue;
+      if (a.nsplit > 1) {
+        float* p = a.part +
+                   (((long)split * a.B * a.Hk + bh) * a.Sk + k) * 2 * DP;
+        p[col] = dk[d][j];
+        p[DP + col] = dv[d][j];
+      } else if (col < a.D) {
+        ((T*)row_ptr<T>(a.dk, b, hk, k))[col] = (T)(dk[d][j] * a.scale);
+        ((T*)row_ptr<T>(a.dv, b, hk, k))[col] = (T)dv[d][j];
+      }
+    }
+}
+
+// sums of the splits' dQ, in the splits' order: a wave a row
+template <typename T>
+__global__ __launch_bounds__(256) void att_dq_join_kernel(Att a, int DP) {
+  const int M = a.G * a.Sq, l = threadIdx.x & 63;
+  const long rows = (long)a.B * a.Hk * M;
+  const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  const long bh = at / M;
+  T* out = q_row<T>(a.dq, a, bh / a.Hk, (int)(bh % a.Hk),
+                    (int)(at - bh * M));
+  for (int d = l; d < a.D; d += 64) {
+    float v = 0.f;
+    for (int k = 0; k < a.nsplit; ++k) v += a.part[(k * rows + at) * DP + d];
+    out[d] = (T)(v * a.scale);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void att_dkv_join_kernel(Att a, int DP) {
+  const int l = threadIdx.x & 63;
+  const long rows = (long)a.B * a.Hk * a.Sk;
+  const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  const long bh = at / a.Sk;
+  const int key = (int)(at - bh * a.Sk);
+  T* dk = (T*)row_ptr<T>(a.dk, bh / a.Hk, (int)(bh % a.Hk), key);
+  T* dv = (T*)row_ptr<T>(a.dv, bh / a.Hk, (int)(bh % a.Hk), key);
+  for (int d = l; d < a.D; d += 64) {
+    float u = 0.f, v = 0.f;
+    for (int k = 0; k < a.nsplit; ++k) {
+      const float* p = a.part + (k * rows + at) * 2 * DP;
+      u += p[d];
+      v += p[DP + d];
+    }
+    dk[d] = (T)(u * a.scale);
+    dv[d] = (T)v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+int pad_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+// as many splits as bring the launch to about four blocks a CU, but none
+// shorter than `least` tiles
+int splits(long blocks, long tiles, long least) {
+  long n = std::min(1024 / std::max<long>(blocks, 1),
+                    tiles / std::max<long>(least, 1));
+  return (int)std::max<long>(1, std::min<long>(n, 64));
+}
+
+struct Plan {
+  int DP, NW, fwd, dq, dkv, kw;  // waves of rows, splits, waves of keys
+};
+
+// NW = 0: the kernel for single tokens
+Plan make_plan(long B, long H, long Hk, long Sq, long Sk, long D) {
+  Plan p;
+  const long M = H / Hk * Sq, bh = B * Hk;
+  p.DP = pad_dim((int)D);
+  p.NW = M <= 32 ? 0 : M <= 64 ? 2 : 4;
+  const int rows = std::max(p.NW, 1) * 32;
+  const long tiles = (Sk + 63) / 64;
+  p.fwd = splits(bh * ((M + rows - 1) / rows), tiles, p.NW ? 4 : 8);
+  const int qrows = p.NW == 4 ? 128 : 64;
+  p.dq = splits(bh * ((M + qrows - 1) / qrows), tiles, 4);
+  p.kw = Sk <= 64 ? 2 : 4;
+  p.dkv = splits(bh * ((Sk + p.kw * 32 - 1) / (p.kw * 32)), (M + 63) / 64, 4);
+  return p;
+}
+
+struct Heads {
+  long B, S, sb, ss;
+};
+
+// [B, S, ...] or, time first, [S, B, ...]
+Heads lead(const Arr& x, bool tnc, const char* name) {
+  MX_CHECK(x.dim() == 3, name << " must have three axes");
+  const long n = x.size(2), a = x.size(0), b = x.size(1);
+  return tnc ? Heads{b, a, n, b * n} : Heads{a, b, b * n, n};
+}
+
+View view(const Arr& x, const Heads& h, long off, long sh) {
+  return View{(char*)x.ptr + off * dtype_size(x.dtype), h.sb, h.ss, sh};
+}
+
+Att make_att(const Arr& q, const Arr& kv, const Arr& values, int heads,
+             int kv_heads, const Arr& len, const Arr& mask, bool tnc) {
+  const char* name = "encdec_attention";
+  const Heads hq = lead(q, tnc, name), hk = lead(kv, tnc, name);
+  MX_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
+           name << ": kv_heads must divide heads");
+  MX_CHECK(q.size(2) % heads == 0, name << ": heads must divide the queries");
+  const long D = q.size(2) / heads;
+  MX_CHECK(D >= 1 && D <= 128, name << ": head sizes of 1 to 128, got " << D);
+  MX_CHECK(hq.B == hk.B && kv.dtype == q.dtype &&
+               kv.size(2) == kv_heads * D * (values.defined() ? 1 : 2),
+           name << ": the keys do not fit the queries and heads");
+  if (values.defined()) {
+    const Heads hv = lead(values, tnc, name);
+    MX_CHECK(hv.B == hk.B && hv.S == hk.S && values.size(2) == kv.size(2) &&
+                 values.dtype == kv.dtype,
+             name << ": the values must be like the keys");
+  }
+  MX_CHECK(!len.defined() || (len.dtype == kInt32 && len.numel() == hq.B),
+           name << ": valid_length must hold one int32 for each sequence");
+  MX_CHECK(!mask.defined() || ((mask.dtype == kUint8 || mask.dtype == kBool) &&
+                               mask.numel() == hk.B * hk.S),
+           name << ": the mask must hold one byte for each key");
+  MX_CHECK(hq.S * heads < (1L << 30) && hk.S < (1L << 30) &&
+               hq.B * heads < (1L << 30),
+           name << ": too many rows, keys or sequences");
+  Att a = {};
+  a.q = view(q, hq, 0, D);
+  if (values.defined()) {
+    a.k = view(kv, hk, 0, D);
+    a.v = view(values, hk, 0, D);
+  } else {
+    a.k = view(kv, hk, 0, 2 * D);
+    a.v = view(kv, hk, D, 2 * D);
+  }
+  a.len = len.data<int>();
+  a.mask = mask.data<uint8_t>();
+  a.B = (int)hq.B;
+  a.H = heads;
+  a.Hk = kv_heads;
+  a.G = heads / kv_heads;
+  a.Sq = (int)hq.S;
+  a.Sk = (int)hk.S;
+  a.D = (int)D;
+  a.nsplit = 1;
+  a.scale = 1.f / sqrtf((float)D);
+  return a;
+}
+
+bool vectors(std::initializer_list<View> vs, int D, size_t size) {
+  if ((D * size) % 16) return false;  // then so are all strides
+  for (auto& v : vs)
+    if ((uintptr_t)v.p & 15) return false;
+  return true;
+}
+
+unsigned grid(long blocks) {
+  MX_CHECK(blocks < (1L << 31), "encdec_attention: too many blocks");
+  return (unsigned)blocks;
+}
+
+template <typename F>
+void by_dim(int DP, F f) {
+  if (DP == 32) f(std::integral_constant<int, 32>{});
+  else if (DP == 64) f(std::integral_constant<int, 64>{});
+  else f(std::integral_constant<int, 128>{});
+}
+
+// keys a tile: 64, and 32 where the tile is of 32-bit values
+template <typename T>
+constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
+
+template <typename T>
+void fwd(const LaunchCtx& lc, Att a, const Plan& p) {
+  constexpr int BN = tile_rows<T>();
+  a.vec = vectors({a.q, a.k, a.v, a.o}, a.D, sizeof(T));
+  a.nsplit = p.fwd;
+  const long bh = (long)a.B * a.Hk, M = (long)a.G * a.Sq;
+  by_dim(p.DP, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    const unsigned n = grid(bh * a.nsplit *
+                            (p.NW ? (M + p.NW * 32 - 1) / (p.NW * 32) : 1));
+    if (p.NW == 0)
+      // a wave's own tile of 16 KB at most
+      att_token_kernel<T, DP, sizeof(T) == 2 && DP <= 64 ? 64 : 32>
+          <<<n, 256, 0, lc.stream>>>(a);
+    else if (p.NW == 2)
+      att_fwd_kernel<T, DP, 2, BN><<<n, 128, 0, lc.stream>>>(a);
+    else
+      att_fwd_kernel<T, DP, 4, BN><<<n, 256, 0, lc.stream>>>(a);
+  });
+  if (a.nsplit > 1)
+    att_join_kernel<T><<<grid((bh * M + 3) / 4), 256, 0, lc.stream>>>(a, p.DP);
+}
+
+template <typename T>
+void bwd(const LaunchCtx& lc, Att a, const Plan& p) {
+  constexpr int BN = tile_rows<T>();
+  a.vec = vectors({a.q, a.k, a.v, a.dout, a.dq}, a.D, sizeof(T));
+  const long bh = (long)a.B * a.Hk, M = (long)a.G * a.Sq;
+  if (M) {
+    att_delta_kernel<T><<<grid((bh * M + 3) / 4), 256, 0, lc.stream>>>(a);
+    a.nsplit = p.dq;
+    by_dim(p.DP, [&](auto dp) {
+      constexpr int DP = decltype(dp)::value;
+      if (p.NW == 4)
+        att_dq_kernel<T, DP, 4, BN>
+            <<<grid(bh * a.nsplit * ((M + 127) / 128)), 256, 0, lc.stream>>>(
+                a);
+      else
+        att_dq_kernel<T, DP, 2, BN>
+            <<<grid(bh * a.nsplit * ((M + 63) / 64)), 128, 0, lc.stream>>>(a);
+    });
+    if (a.nsplit > 1)
+      att_dq_join_kernel<T>
+          <<<grid((bh * M + 3) / 4), 256, 0, lc.stream>>>(a, p.DP);
+  }
+  if (a.Sk) {
+    a.nsplit = p.dkv;
+    by_dim(p.DP, [&](auto dp) {
+      constexpr int DP = decltype(dp)::value;
+      const int keys = p.kw * 32;
+      const unsigned n = grid(bh * a.nsplit * ((a.Sk + keys - 1) / keys));
+      if (p.kw == 4)
+        att_dkv_kernel<T, DP, 4, BN><<<n, 256, 0, lc.stream>>>(a);
+      else
+        att_dkv_kernel<T, DP, 2, BN><<<n, 128, 0, lc.stream>>>(a);
+    });
+    if (a.nsplit > 1)
+      att_dkv_join_kernel<T>
+          <<<grid((bh * a.Sk + 3) / 4), 256, 0, lc.stream>>>(a, p.DP);
+  }
+}
+
+// the partial results behind delta start at 16 bytes
+int64_t align4(int64_t n) { return (n + 3) & ~(int64_t)3; }
+
+}  // namespace
+
+std::vector<int64_t> encdec_attention_workspace(int64_t B, int64_t H,
+                                                int64_t Hk, int64_t Sq,
+                                                int64_t Sk, int64_t D) {
+  MX_CHECK(H > 0 && Hk > 0 && H % Hk == 0 && D > 0,
+           "encdec_attention: bad heads");
+  const Plan p = make_plan(B, H, Hk, Sq, Sk, D);
+  const int64_t rows = B * H * Sq;
+  const int64_t fwd = p.fwd > 1 ? p.fwd * rows * (p.DP + 2) : 0;
+  const int64_t dq = p.dq > 1 ? p.dq * rows * p.DP : 0;
+  const int64_t dkv = p.dkv > 1 ? p.dkv * B * Hk * Sk * 2 * p.DP : 0;
+  // the two splits of the backward use the workspace one after the other
+  return {fwd, align4(rows) + std::max(dq, dkv)};
+}
+
+void encdec_attention_fwd_raw(const LaunchCtx& lc, const Arr& q,
+                              const Arr& kv, const Arr& values, int heads,
+                              int kv_heads, const Arr& len, const Arr& mask,
+                              bool tnc, const Arr& out, const Arr& lse,
+                              const Arr& work) {
+  if (out.numel() == 0) return;
+  Att a = make_att(q, kv, values, heads, kv_heads, len, mask, tnc);
+  const Plan p = make_plan(a.B, a.H, a.Hk, a.Sq, a.Sk, a.D);
+  MX_CHECK(out.shape == q.shape && out.dtype == q.dtype,
+           "encdec_attention: the output must be like the queries");
+  MX_CHECK(!lse.defined() ||
+               (lse.dtype == kFloat32 && lse.numel() == (long)a.B * a.H * a.Sq),
+           "encdec_attention: one float32 for each row of each head");
+  MX_CHECK((work.defined() && work.dtype == kFloat32 ? work.numel() : 0) >=
+               encdec_attention_workspace(a.B, a.H, a.Hk, a.Sq, a.Sk,
+                                          a.D)[0],
+           "encdec_attention: workspace too small");
+  a.o = view(out, lead(out, tnc, "out"), 0, a.D);
+  a.lse = lse.data<float>();
+  a.part = work.data<float>();
+  DISPATCH_FLOAT_NATIVE(q.dtype, "encdec_attention",
+                        [&] { fwd<scalar_t>(lc, a, p); });
+  HIP_CHECK_LAST();
+}
+
+void encdec_attention_bwd_raw(const LaunchCtx& lc, const Arr& dout,
+                              const Arr& q, const Arr& kv, const Arr& values,
+                              int heads, int kv_heads, const Arr& len,
+                              const Arr& mask, bool tnc, const Arr& out,
+                              const Arr& lse, const Arr& dq, const Arr& dkv,
+                              const Arr& dvalues, const Arr& work) {
+  if (dkv.numel() == 0 && dq.numel() == 0) return;
+  Att a = make_att(q, kv, values, heads, kv_heads, len, mask, tnc);
+  const Plan p = make_plan(a.B, a.H, a.Hk, a.Sq, a.Sk, a.D);
+  MX_CHECK(dout.shape == q.shape && dout.dtype == q.dtype &&
+               out.shape == q.shape && out.dtype == q.dtype &&
+               dq.shape == q.shape && dq.dtype == q.dtype &&
+               dkv.shape == kv.shape && dkv.dtype == kv.dtype &&
+               values.defined() == dvalues.defined() &&
+               (!values.defined() || (dvalues.shape == values.shape &&
+                                      dvalues.dtype == values.dtype)),
+           "encdec_attention backward: a gradient must be like its input");
+  const long rows = (long)a.B * a.H * a.Sq;
+  MX_CHECK(rows == 0 || (lse.dtype == kFloat32 && lse.numel() == rows),
+           "encdec_attention backward: one float32 for each row");
+  MX_CHECK((work.defined() && work.dtype == kFloat32 ? work.numel() : 0) >=
+               encdec_attention_workspace(a.B, a.H, a.Hk, a.Sq, a.Sk,
+                                          a.D)[1],
+           "encdec_attention backward: workspace too small");
+  a.o = view(out, lead(out, tnc, "out"), 0, a.D);
+  a.dout = view(dout, lead(dout, tnc, "dout"), 0, a.D);
+  a.dq = view(dq, lead(dq, tnc, "dq"), 0, a.D);
+  const Heads hk = lead(dkv, tnc, "dkv");
+  if (values.defined()) {
+    a.dk = view(dkv, hk, 0, a.D);
+    a.dv = view(dvalues, hk, 0, a.D);
+  } else {
+    a.dk = view(dkv, hk, 0, 2 * a.D);
+    a.dv = view(dkv, hk, a.D, 2 * a.D);
+  }
+  a.lse = lse.data<float>();
+  a.delta = work.data<float>();
+  a.part = work.data<float>() + align4(rows);
+  DISPATCH_FLOAT_NATIVE(q.dtype, "encdec_attention backward",
+                        [&] { bwd<scalar_t>(lc, a, p); });
+  HIP_CHECK_LAST();
+}
+
+}  // namespace mxcore

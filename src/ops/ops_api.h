@@ -83,6 +83,26 @@ void rms_norm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
                       const Arr& h, const Arr& gamma, const Arr& rstd,
                       const Arr& dx, const Arr& dgamma, const Arr& partial);
 
+// ---- encdec_attention.hip -------------------------------------------------
+// q [B,Sq,heads*D] over kv [B,Sk,kv_heads*2*D] (a head's key, then its value;
+// or keys and values apart), tnc: [S,B,..].  len int32 [B], mask byte [B,Sk],
+// lse fp32 [B,heads,Sq] (optional), work: fp32 of the sizes that
+// encdec_attention_workspace gives, {forward, backward}
+std::vector<int64_t> encdec_attention_workspace(int64_t B, int64_t H,
+                                                int64_t Hk, int64_t Sq,
+                                                int64_t Sk, int64_t D);
+void encdec_attention_fwd_raw(const LaunchCtx& lc, const Arr& q,
+                              const Arr& kv, const Arr& values, int heads,
+                              int kv_heads, const Arr& len, const Arr& mask,
+                              bool tnc, const Arr& out, const Arr& lse,
+                              const Arr& work);
+void encdec_attention_bwd_raw(const LaunchCtx& lc, const Arr& dout,
+                              const Arr& q, const Arr& kv, const Arr& values,
+                              int heads, int kv_heads, const Arr& len,
+                              const Arr& mask, bool tnc, const Arr& out,
+                              const Arr& lse, const Arr& dq, const Arr& dkv,
+                              const Arr& dvalues, const Arr& work);
+
 // ---- conv.hip (NHWC) ------------------------------------------------------
 void conv2d_fwd_raw(const LaunchCtx& lc, const Arr& x, const Arr& w,
                     const Arr& bias, int sh, int sw, int ph, int pw, int dh,
