@@ -1,4 +1,5 @@
-"""Contrib operators: attention over an encoder's states, and control flow.
+"""Contrib operators: attention over an encoder's states, sampling of tokens,
+and control flow.
 
 Control-flow operators (reference src/operator/control_flow.cc:
 ``_foreach``, ``_while_loop``, ``_cond`` and python wrappers
@@ -12,9 +13,10 @@ import torch
 
 from .ndarray import NDArray
 from ..ops import contrib_transformer as _ct
+from ..ops import sampling as _sampling
 
 __all__ = ['foreach', 'while_loop', 'cond', 'isinf', 'isnan', 'isfinite',
-           'encdec_attention']
+           'encdec_attention', 'sample_tokens']
 
 
 def _as_list(x):
@@ -112,3 +114,30 @@ def encdec_attention(queries, keys_values, values=None, heads=1,
     return NDArray(_ct.encdec_attention(t(queries), t(keys_values), t(values),
                                         heads, kv_heads, t(valid_length),
                                         t(mask), layout))
+
+
+def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0, get_prob=False):
+    """The next token of each row of ``logits`` (N, V), drawn with the given
+    random numbers ``uniform`` (N,) float32 in [0, 1).
+
+    In the order of the logits, the largest first (of equal ones the lower
+    index first), with weights exp((logit - max) / temperature): the first
+    ``top_k`` are kept (0: all), of those the shortest prefix that holds
+    ``top_p`` of their sum, of those the ones with at least ``min_p`` of the
+    largest weight; the token is the first whose running sum exceeds uniform
+    times the kept sum.  A temperature of 0 takes the largest logit.  Each
+    parameter is a number, or an array of one for each row (float32, top_k
+    int32; there a temperature that is not positive counts as 0).  A NaN is
+    never drawn; a row without a finite or infinite logit gives -1.
+
+    Returns int32 tokens (N,), or with ``get_prob`` ``[tokens, logp]``: the
+    token's log-probability among the kept ones.  float16, bfloat16 and
+    float32 logits, up to 2^19 a row; sums in 64 bits, the same at every call.
+    """
+    def t(x):
+        return x._t if isinstance(x, NDArray) else x
+    token, logp = _sampling.sample_tokens(
+        logits._t, uniform._t, t(temperature), t(top_k), t(top_p), t(min_p),
+        get_prob)
+    return [NDArray(token), NDArray(logp)] if get_prob else NDArray(token)

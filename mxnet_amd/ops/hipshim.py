@@ -621,6 +621,26 @@ def embedding_bwd(indices, dy, vocab):
     return dw
 
 
+def sample_tokens(logits, uniform, temperature, top_k, top_p, min_p,
+                  want_logp):
+    """Each parameter is a number or a tensor of one a row."""
+    logits = _c(logits)
+    dev, s = _dev_stream(logits)
+    N, V = logits.shape
+    token = torch.empty((N,), dtype=torch.int32, device=logits.device)
+    logp = torch.empty((N,), dtype=torch.float32, device=logits.device) \
+        if want_logp else None
+    n = _raw.sample_tokens_workspace(N, V)
+    work = torch.empty((n,), dtype=torch.uint8, device=logits.device) \
+        if n else None
+    ps = (temperature, top_k, top_p, min_p)
+    arrays = [_arr(p) if isinstance(p, torch.Tensor) else None for p in ps]
+    numbers = [0 if isinstance(p, torch.Tensor) else p for p in ps]
+    _raw.sample_tokens(dev, s, _arr(logits), _arr(uniform), *arrays, *numbers,
+                       _arr(token), _arr(logp), _arr(work))
+    return token, logp
+
+
 # ---------------------------------------------------------------------------
 # int8
 # ---------------------------------------------------------------------------

@@ -220,6 +220,18 @@ void init_raw(py::module_& m) {
                                    ToArr(dq), ToArr(dkv), ToArr(dvalues),
                                    ToArr(work));
         });
+  r.def("sample_tokens_workspace", &sample_tokens_workspace);
+  r.def("sample_tokens",
+        [](int dev, uintptr_t stream, py::handle logits, py::handle u,
+           py::handle temperature, py::handle top_k, py::handle top_p,
+           py::handle min_p, double t, int64_t k, double p, double m,
+           py::handle token, py::handle logp, py::handle work) {
+          Launch l(dev, stream);
+          sample_tokens_raw(l.lc, ToArr(logits), ToArr(u),
+                            ToArr(temperature), ToArr(top_k), ToArr(top_p),
+                            ToArr(min_p), t, k, p, m, ToArr(token),
+                            ToArr(logp), ToArr(work));
+        });
   r.def("conv2d_fwd", [](int dev, uintptr_t stream, py::handle x,
                          py::handle w, py::handle bias, int sh, int sw,
                          int ph, int pw, int dh, int dw, int groups,

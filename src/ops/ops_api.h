@@ -103,6 +103,17 @@ void encdec_attention_bwd_raw(const LaunchCtx& lc, const Arr& dout,
                               const Arr& lse, const Arr& dq, const Arr& dkv,
                               const Arr& dvalues, const Arr& work);
 
+// ---- sample.hip -----------------------------------------------------------
+// token [N] int32 (and logp fp32) from logits [N,V] and numbers u [N]; each
+// parameter is one number, or one a row where its array is defined.  work:
+// bytes of sample_tokens_workspace
+int64_t sample_tokens_workspace(int64_t N, int64_t V);
+void sample_tokens_raw(const LaunchCtx& lc, const Arr& logits, const Arr& u,
+                       const Arr& temperature, const Arr& top_k,
+                       const Arr& top_p, const Arr& min_p, double t,
+                       int64_t k, double p, double m, const Arr& token,
+                       const Arr& logp, const Arr& work);
+
 // ---- conv.hip (NHWC) ------------------------------------------------------
 void conv2d_fwd_raw(const LaunchCtx& lc, const Arr& x, const Arr& w,
                     const Arr& bias, int sh, int sw, int ph, int pw, int dh,
