@@ -14,6 +14,7 @@ import torch
 from .ndarray import NDArray
 from ..ops import contrib_transformer as _ct
 from ..ops import sampling as _sampling
+from . import ops as _ops
 
 __all__ = ['foreach', 'while_loop', 'cond', 'isinf', 'isnan', 'isfinite',
            'encdec_attention', 'sample_tokens']
@@ -109,11 +110,33 @@ def encdec_attention(queries, keys_values, values=None, heads=1,
     without a key gives zeros.  float16, bfloat16 and float32; head sizes up
     to 128 on the GPU.
     """
+    if queries.is_native:
+        return _encdec_native(queries, keys_values, values, heads, kv_heads,
+                              valid_length, mask, layout)
+
     def t(x):
         return None if x is None else x._t
     return NDArray(_ct.encdec_attention(t(queries), t(keys_values), t(values),
                                         heads, kv_heads, t(valid_length),
                                         t(mask), layout))
+
+
+def _encdec_native(queries, keys_values, values, heads, kv_heads,
+                   valid_length, mask, layout):
+    if layout not in ('NTC', 'TNC'):
+        raise ValueError(f'encdec_attention: layout must be NTC or TNC, got '
+                         f'{layout!r}')
+    heads = int(heads)
+    if valid_length is not None and str(valid_length.dtype) == 'int64':
+        valid_length = valid_length.astype('int32')
+    more = [values, valid_length, mask]
+    attrs = {'heads': str(heads),
+             'kv_heads': str(heads if kv_heads is None else int(kv_heads)),
+             'tnc': '1' if layout == 'TNC' else '0'}
+    for name, x in zip(('values', 'length', 'mask'), more):
+        attrs['has_' + name] = '0' if x is None else '1'
+    return _ops._ninv('_contrib_encdec_attention',
+                      [queries, keys_values] + more, attrs, nout=2)[0]
 
 
 def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0,
@@ -135,9 +158,32 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0,
     token's log-probability among the kept ones.  float16, bfloat16 and
     float32 logits, up to 2^19 a row; sums in 64 bits, the same at every call.
     """
+    if logits.is_native:
+        return _sample_native(logits, uniform, temperature, top_k, top_p,
+                              min_p, get_prob)
+
     def t(x):
         return x._t if isinstance(x, NDArray) else x
     token, logp = _sampling.sample_tokens(
         logits._t, uniform._t, t(temperature), t(top_k), t(top_p), t(min_p),
         get_prob)
     return [NDArray(token), NDArray(logp)] if get_prob else NDArray(token)
+
+
+def _sample_native(logits, uniform, temperature, top_k, top_p, min_p,
+                   get_prob):
+    ins, attrs = [logits, uniform], {}
+    for name, value, dtype, low, high in (
+            ('temperature', temperature, 'float32', 0.0, 1e30),
+            ('top_k', top_k, 'int32', 0, (1 << 31) - 1),
+            ('top_p', top_p, 'float32', 0.0, 1.0),
+            ('min_p', min_p, 'float32', 0.0, 1.0)):
+        if isinstance(value, NDArray):
+            ins.append(value if str(value.dtype) == dtype
+                       else value.astype(dtype))
+            attrs['has_' + name] = '1'
+        else:
+            attrs[name] = repr(_sampling.check_number(name, value, dtype, low,
+                                                      high))
+    token, logp = _ops._ninv('_contrib_sample_tokens', ins, attrs, nout=2)
+    return [token, logp] if get_prob else token

@@ -205,11 +205,14 @@ def RMSNorm(data, gamma, residual=None, axis=-1, eps=1e-6, out_type=None,
         if out_type not in (None, 'int8'):
             raise ValueError(f'RMSNorm: out_type must be None or int8, got '
                              f'{out_type!r}')
+        if str(gamma.dtype) != 'float32':
+            gamma = gamma.astype('float32')
         ins = [data, gamma] + ([residual] if residual is not None else [])
         attrs = {'eps': repr(float(eps))}
         if out_type == 'int8':
-            outs = _ninv('_contrib_rms_norm_int8', ins, attrs, nout=3)
-            return outs if residual is not None else outs[:2]
+            q, total, scale = _ninv('_contrib_rms_norm_int8', ins, attrs,
+                                    nout=3)
+            return [q, scale] + ([total] if residual is not None else [])
         outs = _ninv('RMSNorm', ins, attrs, nout=3)
         return outs[:2] if residual is not None else outs[0]
     out = _nn.rms_norm(_t(data), _t(gamma),

@@ -25,7 +25,13 @@ def _param(name, value, n, device, dtype, low, high):
         if value.is_floating_point() != dtype.is_floating_point:
             raise TypeError(f'sample_tokens: {name} of {value.dtype}')
         return value.to(dtype).contiguous()
-    if not dtype.is_floating_point:
+    return check_number(name, value, str(dtype).replace('torch.', ''), low,
+                        high)
+
+
+def check_number(name, value, dtype, low, high):
+    """A parameter that is one number: its value, if it lies in its range."""
+    if dtype == 'int32':
         if int(value) != value:
             raise ValueError(f'sample_tokens: {name} must be a whole number, '
                              f'got {value!r}')
