@@ -57,6 +57,14 @@ template <> struct Mat<float> {
   }
 };
 
+// Waves a SIMD: two where a wave's registers (256 then) hold the `n` operands
+// of a row and its accumulators, which hides most of each wave's latencies
+// behind the other; else one.  32-bit fragments take twice the room.
+template <typename T, int DP>
+constexpr int waves(int n) {
+  return n * DP * (int)sizeof(T) <= 256 ? 2 : 1;
+}
+
 // one [B, S, heads, D] view: strides in elements, D contiguous
 struct View {
   void* p;
@@ -74,6 +82,7 @@ struct Att {
   int nsplit;
   int vec;               // 16-byte accesses
   float scale;           // 1 / sqrt(D)
+  float inv_sq;          // 1 / Sq
 };
 
 // ---------------------------------------------------------------------------
@@ -201,8 +210,28 @@ DEV_INLINE const T* row_ptr(const View& v, long b, int head, int s) {
 // row m of the G * Sq rows that share a key head
 template <typename T>
 DEV_INLINE T* q_row(const View& v, const Att& a, long b, int hk, int m) {
-  const int g = m / a.Sq;
-  return (T*)row_ptr<T>(v, b, hk * a.G + g, m - g * a.Sq);
+  // m / Sq by the reciprocal, at most one off
+  int g = (int)((float)m * a.inv_sq), s = m - g * a.Sq;
+  if (s < 0) {
+    --g;
+    s += a.Sq;
+  } else if (s >= a.Sq) {
+    ++g;
+    s -= a.Sq;
+  }
+  return (T*)row_ptr<T>(v, b, hk * a.G + g, s);
+}
+
+// the value of the lane 32 away, and this lane's: their maximum and sum
+DEV_INLINE float pair_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(
+      __float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+DEV_INLINE float pair_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(
+      __float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 DEV_INLINE int kept_keys(const Att& a, int b) {
@@ -213,24 +242,37 @@ DEV_INLINE int kept_keys(const Att& a, int b) {
 
 // ---------------------------------------------------------------------------
 // staging: NT threads bring ROWS rows of DP elements to registers, then LDS.
-// A key that is masked or past the length is stored as zeros, whatever its
-// memory holds, so that a NaN there meets no product.
+// Every load is done, from a row that exists, and what is not wanted (a row
+// past the end, a masked key, columns from D on) becomes zeros on its way to
+// LDS: loads under a condition would be waited for where the branch ends, and
+// a NaN in a masked key's memory meets no product.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int ROWS, int NT>
 struct Stage {
   using TL = Tile<T, DP>;
-  static constexpr int N = (ROWS * TL::CPR + NT - 1) / NT;
+  static constexpr int N = ROWS * TL::CPR / NT;
+  static_assert(ROWS * TL::CPR % NT == 0, "whole chunks a thread");
   int4_t r[N];
-  // row(i) gives the i-th row's address or null
-  template <typename F>
-  DEV_INLINE void load(F row, int t, int D, bool vec) {
+  unsigned want;  // a bit a chunk
+  // ptr(i): the i-th row, or another that exists; ok(i): whether it is wanted
+  template <typename P, typename K>
+  DEV_INLINE void load(P ptr, K ok, int t, int D, bool vec) {
+    want = 0;
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = i * NT + t;
-      r[i] = int4_t{0, 0, 0, 0};
-      if ((ROWS * TL::CPR) % NT == 0 || c < ROWS * TL::CPR) {
-        const T* p = row(c / TL::CPR);
-        if (p) r[i] = load_chunk<T>(p, (c % TL::CPR) * TL::EPC, D, vec);
+      for (int i = 0; i < N; ++i) {
+        const int row = (i * NT + t) / TL::CPR;
+        const int d = (i * NT + t) % TL::CPR * TL::EPC;
+        r[i] = *(const int4_t*)(ptr(row) + (d < D ? d : 0));
+        if (d < D && ok(row)) want |= 1u << i;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int row = (i * NT + t) / TL::CPR;
+        r[i] = load_chunk<T>(ptr(row), (i * NT + t) % TL::CPR * TL::EPC, D,
+                             false);
+        if (ok(row)) want |= 1u << i;
       }
     }
   }
@@ -238,9 +280,46 @@ struct Stage {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = i * NT + t;
-      if ((ROWS * TL::CPR) % NT == 0 || c < ROWS * TL::CPR)
-        *(int4_t*)(tile + TL::at(c / TL::CPR, c % TL::CPR)) = r[i];
+      const int4_t zero = {0, 0, 0, 0};
+      *(int4_t*)(tile + TL::at(c / TL::CPR, c % TL::CPR)) =
+          want >> i & 1 ? r[i] : zero;
     }
+  }
+};
+
+// the keys and values of one tile; `n` keys are kept (n >= 1), of those the
+// ones whose mask is not 0
+template <typename T, int DP, int BN, int NT>
+struct KeyTiles {
+  Stage<T, DP, BN, NT> k, v;
+  const T *kb, *vb;
+  long ks, vs;
+  const uint8_t* mask;
+  int n;
+  DEV_INLINE KeyTiles(const Att& a, int b, int hk, int kept)
+      : kb(row_ptr<T>(a.k, b, hk, 0)), vb(row_ptr<T>(a.v, b, hk, 0)),
+        ks(a.k.ss), vs(a.v.ss),
+        mask(a.mask ? a.mask + (long)b * a.Sk : nullptr), n(kept) {}
+  DEV_INLINE bool ok(int key) const {
+    return key < n && (!mask || mask[min(key, n - 1)]);
+  }
+  DEV_INLINE void load(int tile, int t, int D, bool vec) {
+    const int k0 = tile * BN;
+    auto good = [&](int r) { return ok(k0 + r); };
+    k.load([&](int r) { return kb + min(k0 + r, n - 1) * ks; }, good, t, D,
+           vec);
+    v.load([&](int r) { return vb + min(k0 + r, n - 1) * vs; }, good, t, D,
+           vec);
+  }
+  DEV_INLINE void store(char* lk, char* lv, uint8_t* keep, int tile,
+                        int t) const {
+    k.store(lk, t);
+    v.store(lv, t);
+    for (int r = t; r < BN; r += NT) keep[r] = ok(tile * BN + r);
+  }
+  // whether a tile has keys that are left out
+  DEV_INLINE bool partial(int tile) const {
+    return mask || (tile + 1) * BN > n;
   }
 };
 
@@ -294,7 +373,7 @@ DEV_INLINE void softmax_step(float16_t (&s)[KB], float16_t (&acc)[DP / 32],
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
-  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  top = pair_max(top);
   // The reference follows the maximum only when that leaves it by more than
   // 2^8: until then the weights are at most 256, which no accumulator
   // minds, and the output is not scaled again
@@ -401,7 +480,7 @@ DEV_INLINE void finish_row(const Att& a, const float16_t (&acc)[DP / 32],
 // forward: NW waves of 32 rows each over tiles of BN keys that all share
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int NW, int BN>
-__global__ __launch_bounds__(NW * 64) void att_fwd_kernel(Att a) {
+__global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_fwd_kernel(Att a) {
   using TL = Tile<T, DP>;
   constexpr int NT = NW * 64, KB = BN / 32, BYTES = BN * TL::RB;
   __shared__ __attribute__((aligned(16))) char lk[2][BYTES], lv[2][BYTES];
@@ -419,7 +498,6 @@ __global__ __launch_bounds__(NW * 64) void att_fwd_kernel(Att a) {
   const int tiles = (n + BN - 1) / BN;
   const int t0 = (int)((long)tiles * split / a.nsplit);
   const int t1 = (int)((long)tiles * (split + 1) / a.nsplit);
-  const uint8_t* mask = a.mask ? a.mask + (long)b * a.Sk : nullptr;
 
   typename Mat<T>::Frag qf[DP / 16];
   const T* qr = row < M ? q_row<T>(a.q, a, b, hk, row) : nullptr;
@@ -429,42 +507,24 @@ __global__ __launch_bounds__(NW * 64) void att_fwd_kernel(Att a) {
   float16_t acc[DP / 32] = {};
   float m = kNegInf, sum = 0.f;
 
-  Stage<T, DP, BN, NT> sk, sv;
-  auto keep = [&](int key) {
-    return key < n && (!mask || mask[key]);
-  };
-  auto fetch = [&](int i) {
-    sk.load([&](int r) {
-      const int key = i * BN + r;
-      return keep(key) ? row_ptr<T>(a.k, b, hk, key) : nullptr;
-    }, t, a.D, vec);
-    sv.load([&](int r) {
-      const int key = i * BN + r;
-      return keep(key) ? row_ptr<T>(a.v, b, hk, key) : nullptr;
-    }, t, a.D, vec);
-  };
-  auto put = [&](int i, int buf) {
-    sk.store(lk[buf], t);
-    sv.store(lv[buf], t);
-    for (int r = t; r < BN; r += NT) lkeep[buf][r] = keep(i * BN + r);
-  };
+  KeyTiles<T, DP, BN, NT> kt(a, b, hk, n);
   if (t0 < t1) {
-    fetch(t0);
-    put(t0, 0);
+    kt.load(t0, t, a.D, vec);
+    kt.store(lk[0], lv[0], lkeep[0], t0, t);
   }
   __syncthreads();
   for (int i = t0; i < t1; ++i) {
     const int buf = (i - t0) & 1;
-    if (i + 1 < t1) fetch(i + 1);
+    if (i + 1 < t1) kt.load(i + 1, t, a.D, vec);
     float16_t s[KB];
     scores<T, DP, KB>(lk[buf], qf, s, l);
-    if (mask || (i + 1) * BN > n) drop_keys<KB>(lkeep[buf], s, h);
+    if (kt.partial(i)) drop_keys<KB>(lkeep[buf], s, h);
     softmax_step<T, DP, KB>(s, acc, m, sum, a.scale * kLog2e);
     weigh<T, DP, KB>(lv[buf], s, acc, l);
-    if (i + 1 < t1) put(i + 1, buf ^ 1);
+    if (i + 1 < t1) kt.store(lk[buf ^ 1], lv[buf ^ 1], lkeep[buf ^ 1], i + 1, t);
     __syncthreads();
   }
-  sum += __shfl_xor(sum, 32, 64);
+  sum = pair_sum(sum);
   finish_row<T, DP>(a, acc, m, sum, split, b, hk, row, h);
 }
 
@@ -474,7 +534,7 @@ __global__ __launch_bounds__(NW * 64) void att_fwd_kernel(Att a) {
 // joined at the end.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int BN>
-__global__ __launch_bounds__(256) void att_token_kernel(Att a) {
+__global__ __launch_bounds__(256, (waves<T, DP>(1))) void att_token_kernel(Att a) {
   using TL = Tile<T, DP>;
   constexpr int NW = 4, KB = BN / 32, BYTES = BN * TL::RB;
   constexpr int JOIN = 32 * (DP + 4) * 4;  // one wave's O^T, m and l
@@ -492,7 +552,6 @@ __global__ __launch_bounds__(256) void att_token_kernel(Att a) {
   const int tiles = (n + BN - 1) / BN, parts = a.nsplit * NW;
   const int t0 = (int)((long)tiles * (split * NW + w) / parts);
   const int t1 = (int)((long)tiles * (split * NW + w + 1) / parts);
-  const uint8_t* mask = a.mask ? a.mask + (long)b * a.Sk : nullptr;
 
   typename Mat<T>::Frag qf[DP / 16];
   const T* qr = row < M ? q_row<T>(a.q, a, b, hk, row) : nullptr;
@@ -503,41 +562,26 @@ __global__ __launch_bounds__(256) void att_token_kernel(Att a) {
   float m = kNegInf, sum = 0.f;
   char *lk = lds[w], *lv = lds[w] + BYTES;
 
-  Stage<T, DP, BN, 64> sk, sv;
-  auto keep = [&](int key) {
-    return key < n && (!mask || mask[key]);
-  };
-  auto fetch = [&](int i) {
-    sk.load([&](int r) {
-      const int key = i * BN + r;
-      return keep(key) ? row_ptr<T>(a.k, b, hk, key) : nullptr;
-    }, l, a.D, vec);
-    sv.load([&](int r) {
-      const int key = i * BN + r;
-      return keep(key) ? row_ptr<T>(a.v, b, hk, key) : nullptr;
-    }, l, a.D, vec);
-  };
-  if (t0 < t1) fetch(t0);
+  KeyTiles<T, DP, BN, 64> kt(a, b, hk, n);
+  if (t0 < t1) kt.load(t0, l, a.D, vec);
   for (int i = t0; i < t1; ++i) {
-    sk.store(lk, l);
-    sv.store(lv, l);
-    if (l < BN) lkeep[w][l] = keep(i * BN + l);
+    kt.store(lk, lv, lkeep[w], i, l);
     // a wave's LDS accesses are done in order; the fence keeps the compiler
     // from moving the reads of other lanes' values over these writes
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (i + 1 < t1) fetch(i + 1);
+    if (i + 1 < t1) kt.load(i + 1, l, a.D, vec);
     float16_t s[KB];
     scores<T, DP, KB>(lk, qf, s, l);
-    if (mask || (i + 1) * BN > n) drop_keys<KB>(lkeep[w], s, h);
+    if (kt.partial(i)) drop_keys<KB>(lkeep[w], s, h);
     softmax_step<T, DP, KB>(s, acc, m, sum, a.scale * kLog2e);
     weigh<T, DP, KB>(lv, s, acc, l);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
-  sum += __shfl_xor(sum, 32, 64);
+  sum = pair_sum(sum);
 
   // join the waves: O^T as rows of DP + 4 values (the pad keeps the 32 rows
   // off each other's banks), then m and l behind them
@@ -611,27 +655,9 @@ __global__ __launch_bounds__(256) void att_join_kernel(Att a, int DP) {
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-// delta = sum_d dO * O: a wave a row
-template <typename T>
-__global__ __launch_bounds__(256) void att_delta_kernel(Att a) {
-  const int M = a.G * a.Sq, l = threadIdx.x & 63;
-  const long rows = (long)a.B * a.Hk * M;
-  const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= rows) return;
-  const long bh = at / M;
-  const int m = (int)(at - bh * M), b = (int)(bh / a.Hk),
-            hk = (int)(bh % a.Hk);
-  const T* o = q_row<T>(a.o, a, b, hk, m);
-  const T* g = q_row<T>(a.dout, a, b, hk, m);
-  float v = 0.f;
-  for (int d = l; d < a.D; d += 64) v += (float)o[d] * (float)g[d];
-  v = wave_reduce_sum(v);
-  if (l == 0) a.delta[at] = v;
-}
-
 // dQ: rows as in the forward, over all keys (or a split's)
 template <typename T, int DP, int NW, int BN>
-__global__ __launch_bounds__(NW * 64) void att_dq_kernel(Att a) {
+__global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att a) {
   using TL = Tile<T, DP>;
   constexpr int NT = NW * 64, KB = BN / 32, BYTES = BN * TL::RB;
   __shared__ __attribute__((aligned(16))) char lk[2][BYTES], lv[2][BYTES];
@@ -649,7 +675,6 @@ __global__ __launch_bounds__(NW * 64) void att_dq_kernel(Att a) {
   const int tiles = (n + BN - 1) / BN;
   const int t0 = (int)((long)tiles * split / a.nsplit);
   const int t1 = (int)((long)tiles * (split + 1) / a.nsplit);
-  const uint8_t* mask = a.mask ? a.mask + (long)b * a.Sk : nullptr;
   const float c = a.scale * kLog2e;
 
   typename Mat<T>::Frag qf[DP / 16], gf[DP / 16];
@@ -661,40 +686,35 @@ __global__ __launch_bounds__(NW * 64) void att_dq_kernel(Att a) {
     gf[ks] = load_frag<T>(gr, ks, h, a.D, vec, row < M);
   }
   const float lse = row < M ? a.lse[(long)bh * M + row] : -kNegInf;
-  const float delta = row < M ? a.delta[(long)bh * M + row] : 0.f;
+  // the row's dO . O, which dK and dV need too
+  float delta = 0.f;
+  {
+    const T* orow = row < M ? q_row<T>(a.o, a, b, hk, row) : nullptr;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const auto of = load_frag<T>(orow, ks, h, a.D, vec, row < M);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta += (float)of[j] * (float)gf[ks][j];
+    }
+    delta = pair_sum(delta);
+    if (split == 0 && h == 0 && row < M)
+      a.delta[(long)bh * M + row] = delta;
+  }
   float16_t acc[DP / 32] = {};
 
-  Stage<T, DP, BN, NT> sk, sv;
-  auto keep = [&](int key) {
-    return key < n && (!mask || mask[key]);
-  };
-  auto fetch = [&](int i) {
-    sk.load([&](int rr) {
-      const int key = i * BN + rr;
-      return keep(key) ? row_ptr<T>(a.k, b, hk, key) : nullptr;
-    }, t, a.D, vec);
-    sv.load([&](int rr) {
-      const int key = i * BN + rr;
-      return keep(key) ? row_ptr<T>(a.v, b, hk, key) : nullptr;
-    }, t, a.D, vec);
-  };
-  auto put = [&](int i, int buf) {
-    sk.store(lk[buf], t);
-    sv.store(lv[buf], t);
-    for (int k = t; k < BN; k += NT) lkeep[buf][k] = keep(i * BN + k);
-  };
+  KeyTiles<T, DP, BN, NT> kt(a, b, hk, n);
   if (t0 < t1) {
-    fetch(t0);
-    put(t0, 0);
+    kt.load(t0, t, a.D, vec);
+    kt.store(lk[0], lv[0], lkeep[0], t0, t);
   }
   __syncthreads();
   for (int i = t0; i < t1; ++i) {
     const int buf = (i - t0) & 1;
-    if (i + 1 < t1) fetch(i + 1);
+    if (i + 1 < t1) kt.load(i + 1, t, a.D, vec);
     float16_t s[KB], dp[KB];
     scores<T, DP, KB>(lk[buf], qf, s, l);
     scores<T, DP, KB>(lv[buf], gf, dp, l);
-    if (mask || (i + 1) * BN > n) drop_keys<KB>(lkeep[buf], s, h);
+    if (kt.partial(i)) drop_keys<KB>(lkeep[buf], s, h);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -702,7 +722,7 @@ __global__ __launch_bounds__(NW * 64) void att_dq_kernel(Att a) {
         s[kb][j] = __builtin_amdgcn_exp2f(fmaf(s[kb][j], c, -lse)) *
                    (dp[kb][j] - delta);
     weigh<T, DP, KB>(lk[buf], s, acc, l);
-    if (i + 1 < t1) put(i + 1, buf ^ 1);
+    if (i + 1 < t1) kt.store(lk[buf ^ 1], lv[buf ^ 1], lkeep[buf ^ 1], i + 1, t);
     __syncthreads();
   }
   if (row >= M) return;
@@ -715,7 +735,7 @@ __global__ __launch_bounds__(NW * 64) void att_dq_kernel(Att a) {
 
 // dK and dV: NW waves of 32 keys each over tiles of BM rows (or a split's)
 template <typename T, int DP, int NW, int BM>
-__global__ __launch_bounds__(NW * 64) void att_dkv_kernel(Att a) {
+__global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att a) {
   using TL = Tile<T, DP>;
   constexpr int NT = NW * 64, BYTES = BM * TL::RB;
   __shared__ __attribute__((aligned(16))) char lq[2][BYTES], lg[2][BYTES];
@@ -749,14 +769,13 @@ __global__ __launch_bounds__(NW * 64) void att_dkv_kernel(Att a) {
 
   Stage<T, DP, BM, NT> sq, sg;
   auto fetch = [&](int i) {
+    auto ok = [&](int rr) { return i * BM + rr < M; };
     sq.load([&](int rr) -> const T* {
-      const int m = i * BM + rr;
-      return m < M ? q_row<T>(a.q, a, b, hk, m) : nullptr;
-    }, t, a.D, vec);
+      return q_row<T>(a.q, a, b, hk, min(i * BM + rr, M - 1));
+    }, ok, t, a.D, vec);
     sg.load([&](int rr) -> const T* {
-      const int m = i * BM + rr;
-      return m < M ? q_row<T>(a.dout, a, b, hk, m) : nullptr;
-    }, t, a.D, vec);
+      return q_row<T>(a.dout, a, b, hk, min(i * BM + rr, M - 1));
+    }, ok, t, a.D, vec);
   };
   auto put = [&](int i, int buf) {
     sq.store(lq[buf], t);
@@ -876,10 +895,10 @@ __global__ __launch_bounds__(256) void att_dkv_join_kernel(Att a, int DP) {
 // ---------------------------------------------------------------------------
 int pad_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// as many splits as bring the launch to about four blocks a CU, but none
+// as many splits as bring the launch to about two blocks a CU, but none
 // shorter than `least` tiles
 int splits(long blocks, long tiles, long least) {
-  long n = std::min(1024 / std::max<long>(blocks, 1),
+  long n = std::min(512 / std::max<long>(blocks, 1),
                     tiles / std::max<long>(least, 1));
   return (int)std::max<long>(1, std::min<long>(n, 64));
 }
@@ -965,6 +984,7 @@ Att make_att(const Arr& q, const Arr& kv, const Arr& values, int heads,
   a.D = (int)D;
   a.nsplit = 1;
   a.scale = 1.f / sqrtf((float)D);
+  a.inv_sq = hq.S ? 1.f / (float)hq.S : 0.f;
   return a;
 }
 
@@ -987,18 +1007,20 @@ void by_dim(int DP, F f) {
   else f(std::integral_constant<int, 128>{});
 }
 
-// keys a tile: 64, and 32 where the tile is of 32-bit values
-template <typename T>
-constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
+// rows a tile of `n` operands in registers: 64, or 32 where those, the tile on
+// its way and the accumulators would not fit the registers of two waves
+template <typename T, int DP>
+constexpr int tile_rows(int n) {
+  return n * DP * (int)sizeof(T) <= 256 && sizeof(T) == 2 ? 64 : 32;
+}
 
 template <typename T>
 void fwd(const LaunchCtx& lc, Att a, const Plan& p) {
-  constexpr int BN = tile_rows<T>();
   a.vec = vectors({a.q, a.k, a.v, a.o}, a.D, sizeof(T));
   a.nsplit = p.fwd;
   const long bh = (long)a.B * a.Hk, M = (long)a.G * a.Sq;
   by_dim(p.DP, [&](auto dp) {
-    constexpr int DP = decltype(dp)::value;
+    constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>(1);
     const unsigned n = grid(bh * a.nsplit *
                             (p.NW ? (M + p.NW * 32 - 1) / (p.NW * 32) : 1));
     if (p.NW == 0)
@@ -1016,14 +1038,12 @@ void fwd(const LaunchCtx& lc, Att a, const Plan& p) {
 
 template <typename T>
 void bwd(const LaunchCtx& lc, Att a, const Plan& p) {
-  constexpr int BN = tile_rows<T>();
-  a.vec = vectors({a.q, a.k, a.v, a.dout, a.dq}, a.D, sizeof(T));
+  a.vec = vectors({a.q, a.k, a.v, a.o, a.dout, a.dq}, a.D, sizeof(T));
   const long bh = (long)a.B * a.Hk, M = (long)a.G * a.Sq;
   if (M) {
-    att_delta_kernel<T><<<grid((bh * M + 3) / 4), 256, 0, lc.stream>>>(a);
     a.nsplit = p.dq;
     by_dim(p.DP, [&](auto dp) {
-      constexpr int DP = decltype(dp)::value;
+      constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>(2);
       if (p.NW == 4)
         att_dq_kernel<T, DP, 4, BN>
             <<<grid(bh * a.nsplit * ((M + 127) / 128)), 256, 0, lc.stream>>>(
@@ -1039,7 +1059,7 @@ void bwd(const LaunchCtx& lc, Att a, const Plan& p) {
   if (a.Sk) {
     a.nsplit = p.dkv;
     by_dim(p.DP, [&](auto dp) {
-      constexpr int DP = decltype(dp)::value;
+      constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>(2);
       const int keys = p.kw * 32;
       const unsigned n = grid(bh * a.nsplit * ((a.Sk + keys - 1) / keys));
       if (p.kw == 4)
