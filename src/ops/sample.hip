@@ -7,16 +7,17 @@
 //   token: the first in the order whose running sum exceeds u * (kept sum)
 //
 // Every step asks for a prefix of one order, so the row is never sorted: it is
-// counted into 2048 buckets of (max - x) / T, 1/64 wide (the weight of each,
-// and for top_k the number), which answers every question up to one bucket;
-// only that bucket's few entries are gathered, sorted and looked at one by one.
+// counted into 4096 buckets of the weight's logarithm, 1/64 octave wide (the
+// weight of each, and for top_k the number), whose running sums answer every
+// question up to one bucket or two.  One scan gathers the entries of all
+// those buckets, and only they are sorted and looked at one by one.
 //
 // Weights are 64-bit: whether a token is kept or drawn lies next to a border.
 // They are counted as whole numbers of 2^-s (s = 62 - ceil(log2 V), at most
 // 51), so that sums cannot overflow and do not depend on the order in which
 // lanes and blocks add.
 //
-// Bound by latency for few rows and by the 64-bit exponentials for many.  The
+// Bound by latency for few rows and by the 64-bit weights for many.  The
 // logits are read from memory once and scanned again from the cache.  Rows
 // that fill the chip, and short ones, take one launch with a block a row; else
 // two launches cut each row into parts for the maximum and the counts, and a
@@ -26,10 +27,10 @@
 namespace mxcore {
 namespace {
 
-constexpr int NB = 2048;      // buckets
-constexpr float STEP = 64.f;  // buckets for each unit of (max - x) / T
-constexpr int LIST = 2048;    // entries that are sorted in LDS
-constexpr int NT = 1024;      // threads of the block that answers for a row
+constexpr int NB = 4096;    // buckets
+constexpr int STEP = 64;    // buckets for each halving of the weight
+constexpr int LIST = 2048;  // entries that are sorted in LDS
+constexpr int NT = 1024;    // threads of the block that answers for a row
 constexpr float kInf = __builtin_huge_valf();
 typedef unsigned long long u64;
 
@@ -53,77 +54,111 @@ struct Sample {
 };
 
 struct Row {
+  double top;    // the maximum; above all float32 where that is infinite
+  double scale;  // buckets for each unit of logit
   double inv;    // 1 / T
-  float finv;    // buckets for each unit of logit
-  float top;
+  float ftop;
   bool greedy;
 };
 
-// NaN counts as -inf: it is never drawn
-template <typename T>
-DEV_INLINE float logit(T x) {
-  const float v = (float)x;
-  return v == v ? v : -kInf;
-}
-
-// f(index, logit) over [i0, i1) by the block's threads, 16 bytes at a time
-// where the memory is aligned
-template <typename T, int THREADS, typename F>
-DEV_INLINE void scan(const T* x, long i0, long i1, F f) {
+// f(index, 16 bytes of logits) and g(index, logit) over [i0, i1) by the
+// block's threads, the first where the memory is aligned.  (Four loads on
+// their way at once gained nothing at 256 rows of 131072, whose 16 waves hide
+// them, and lost 4 us at 32 rows of 30522 to the longer code.)
+template <typename T, int THREADS, typename F, typename G>
+DEV_INLINE void scan_vectors(const T* x, long i0, long i1, F f, G g) {
   constexpr int N = 16 / sizeof(T);
   using VecT = T __attribute__((ext_vector_type(N)));
-  long a = i0 + ((-(uintptr_t)(x + i0) & 15) / sizeof(T));
-  if (a > i1) a = i1;
+  const long a =
+      min(i1, i0 + (long)((-(uintptr_t)(x + i0) & 15) / sizeof(T)));
   const long nv = (i1 - a) / N;
-  for (long i = i0 + threadIdx.x; i < a; i += THREADS) f(i, logit(x[i]));
-  for (long k = threadIdx.x; k < nv; k += THREADS) {
-    const VecT v = *(const VecT*)(x + a + k * N);
-#pragma unroll
-    for (int j = 0; j < N; ++j) f(a + k * N + j, logit(v[j]));
-  }
+  for (long i = i0 + threadIdx.x; i < a; i += THREADS) g(i, (float)x[i]);
+  for (long k = threadIdx.x; k < nv; k += THREADS)
+    f(a + k * N, *(const VecT*)(x + a + k * N));
   for (long i = a + nv * N + threadIdx.x; i < i1; i += THREADS)
-    f(i, logit(x[i]));
+    g(i, (float)x[i]);
 }
 
-// non-increasing in v, so buckets follow the order
-DEV_INLINE int bucket(float v, const Row& r) {
-  if (v == r.top) return 0;
-  const float b = (r.top - v) * r.finv;
-  return b < (float)(NB - 1) ? (int)b : NB - 1;  // NaN (inf * 0): the last
+// f(index, logit) over [i0, i1)
+template <typename T, int THREADS, typename F>
+DEV_INLINE void scan(const T* x, long i0, long i1, F f) {
+  scan_vectors<T, THREADS>(x, i0, i1, [&](long i, auto v) {
+#pragma unroll
+    for (int j = 0; j < (int)(16 / sizeof(T)); ++j) f(i + j, (float)v[j]);
+  }, f);
 }
 
-// (max - x) / T; 0 for an infinite maximum itself
+// f(index, logit) for the few logits of the row that `some` picks: those of 16
+// bytes are looked at without a branch, and then one by one
+template <typename T, int THREADS, typename S, typename F>
+DEV_INLINE void scan_some(const T* x, long n, S some, F f) {
+  scan_vectors<T, THREADS>(x, 0, n, [&](long i, auto v) {
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < (int)(16 / sizeof(T)); ++j)
+      m |= (unsigned)some((float)v[j]) << j;
+    while (m) {
+      const int j = __ffs(m) - 1;
+      m &= m - 1;
+      // the j-th of the vector, by its 32-bit words
+      union {
+        decltype(v) v;
+        unsigned w[4];
+      } u = {v};
+      constexpr int P = 4 / sizeof(T);
+      const int k = j / P;
+      union {
+        unsigned w;
+        T t[P];
+      } e = {k == 0 ? u.w[0] : k == 1 ? u.w[1] : k == 2 ? u.w[2] : u.w[3]};
+      if (P == 2) e.w >>= 16 * (j & 1);
+      f(i + j, (float)e.t[0]);
+    }
+  }, [&](long i, float v) {
+    if (some(v)) f(i, v);
+  });
+}
+
+// How far a logit lies below the maximum, in buckets: -64 log2 of its weight,
+// at most 8000 (which weighs nothing), also for -inf and NaN.  Not increasing
+// in v, so that buckets follow the order.
 DEV_INLINE double depth(float v, const Row& r) {
-  if (v == r.top) return 0.0;
-  return r.greedy ? (double)kInf : ((double)r.top - (double)v) * r.inv;
+  return fmax(fmin((r.top - (double)v) * r.scale, 8000.0), 0.0);
 }
 
-// 2^s exp(-d), rounded to a whole number: exp(-d) = 2^-n e^r with |r| <=
-// ln(2) / 2, e^r by its Taylor series to the 11th power (off by 7e-15, a
-// quarter of 2^-s at 10^5 logits).  Adding 2^52 (1.5 * 2^52 where the number
-// may be negative) rounds a double to a whole number in its lowest bits.
-DEV_INLINE u64 weight(double d, int sbits) {
-  if (!(d < 45.0)) return 0;  // under 2^-64
-  const double t = fma(d, 1.4426950408889634, 0x1.8p52), n = t - 0x1.8p52;
-  // ln 2 to 107 bits, as two doubles
-  double r = fma(n, 0.6931471805599453, -d);
-  r = fma(n, 2.3190468138462996e-17, r);
-  double e = 1.0 / 39916800.0;
-  e = fma(e, r, 1.0 / 3628800.0);
-  e = fma(e, r, 1.0 / 362880.0);
-  e = fma(e, r, 1.0 / 40320.0);
-  e = fma(e, r, 1.0 / 5040.0);
-  e = fma(e, r, 1.0 / 720.0);
-  e = fma(e, r, 1.0 / 120.0);
-  e = fma(e, r, 1.0 / 24.0);
-  e = fma(e, r, 1.0 / 6.0);
-  e = fma(e, r, 0.5);
-  e = fma(e, r, 1.0);
-  e = fma(e, r, 1.0);
-  // 2^(s - n); n is t's lowest bits
-  const int x = 1023 + sbits - (int)__double2loint(t);
-  const double f = __hiloint2double(x << 20, 0);
-  return (u64)__double_as_longlong(fma(e, f, 0x1p52)) - 0x4330000000000000ull;
+// Adding 1.5 * 2^52 rounds a double to a whole number in its lowest bits
+struct Whole {
+  int n;
+  double f;
+};
+DEV_INLINE Whole whole(double d) {
+  const double t = d + 0x1.8p52;
+  return {(int)__double2loint(t), t - 0x1.8p52};
+}
+
+DEV_INLINE int bucket(double d) { return min(whole(d).n, NB - 1); }
+
+// 2^s 2^(-d / 64), rounded to a whole number.  d = 64 q + j + f with |f| <=
+// 1/2: 2^-q is an exponent, 2^(-j / 64) comes from the table and 2^(-f / 64)
+// from its Taylor series to the 4th power (off by 4e-14 / 256 at most: the
+// powers of ln(2) / 128).  Adding 2^52 rounds it.
+DEV_INLINE u64 weight(double d, int sbits, const double* table) {
+  const Whole w = whole(d);
+  const double f = (w.f - d) * 0.010830424696249145;  // ln(2) / 64
+  double e = 1.0 / 120.0;
+  e = fma(e, f, 1.0 / 24.0);
+  e = fma(e, f, 1.0 / 6.0);
+  e = fma(e, f, 0.5);
+  e = fma(e, f, 1.0);
+  e = fma(e, f, 1.0);
+  e *= table[w.n & (STEP - 1)];
+  const double p =
+      __hiloint2double((1023 + sbits - (w.n / STEP)) << 20, 0);
+  return (u64)__double_as_longlong(fma(e, p, 0x1p52)) - 0x4330000000000000ull;
+}
+
+DEV_INLINE void fill_table(double* table) {
+  if (threadIdx.x < STEP) table[threadIdx.x] = exp2(threadIdx.x / -64.0);
 }
 
 // the order as ascending numbers: larger logits first, then lower indices
@@ -146,9 +181,10 @@ DEV_INLINE double temperature(const Sample& a, int n) {
 DEV_INLINE Row make_row(double temp, float top) {
   Row r;
   r.greedy = !(temp > 0.0);
-  r.inv = r.greedy ? 0.0 : 1.0 / temp;
-  r.finv = r.greedy ? kInf : (float)(r.inv * STEP);
-  r.top = top;
+  r.inv = r.greedy ? 1e300 : 1.0 / temp;
+  r.scale = r.greedy ? 1e300 : r.inv * (STEP * 1.4426950408889634);
+  r.top = top == kInf ? 0x1p129 : (double)top;
+  r.ftop = top;
   return r;
 }
 
@@ -185,14 +221,20 @@ DEV_INLINE float parts_top(const Sample& a, int n) {
 // 2. number and weight of each bucket
 template <int THREADS, typename T>
 DEV_INLINE void count_row(const Sample& a, const T* x, long i0, long i1,
-                          const Row& r, bool number, u64* mass,
-                          unsigned* count) {
-  scan<T, THREADS>(x, i0, i1, [&](long, float v) {
-    const int b = bucket(v, r);
-    if (number) atomicAdd(&count[b], 1u);
-    const u64 w = weight(depth(v, r), a.sbits);
-    if (w) atomicAdd(&mass[b], w);
-  });
+                          const Row& r, bool number, const double* table,
+                          u64* mass, unsigned* count) {
+  // (nothing in the loop branches, so that the logits' chains of 64-bit
+  // operations overlap)
+  auto each = [&](auto numbers) {
+    scan<T, THREADS>(x, i0, i1, [&](long, float v) {
+      const double d = depth(v, r);
+      const int b = bucket(d);
+      if (decltype(numbers)::value) atomicAdd(&count[b], 1u);
+      atomicAdd(&mass[b], weight(d, a.sbits, table));
+    });
+  };
+  if (number) each(std::true_type{});
+  else each(std::false_type{});
 }
 
 // how many the row may keep; 0: all.  The numbers are counted only for this
@@ -202,21 +244,23 @@ DEV_INLINE int number_kept(const Sample& a, int n, const Row& r) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void sample_count_kernel(Sample a) {
+__global__ __launch_bounds__(512) void sample_count_kernel(Sample a) {
   __shared__ u64 mass[NB];
   __shared__ unsigned count[NB];
+  __shared__ double table[STEP];
+  fill_table(table);
   const int n = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
-  for (int b = threadIdx.x; b < NB; b += 256) {
+  for (int b = threadIdx.x; b < NB; b += 512) {
     mass[b] = 0;
     count[b] = 0;
   }
   const Row r = make_row(temperature(a, n), parts_top(a, n));
   __syncthreads();
-  count_row<256>(a, (const T*)a.x + n * a.V, a.V * part / a.parts,
+  count_row<512>(a, (const T*)a.x + n * a.V, a.V * part / a.parts,
                  a.V * (part + 1) / a.parts, r, number_kept(a, n, r) != 0,
-                 mass, count);
+                 table, mass, count);
   __syncthreads();
-  for (int b = threadIdx.x; b < NB; b += 256) {
+  for (int b = threadIdx.x; b < NB; b += 512) {
     if (count[b]) atomicAdd(&a.count[(long)n * NB + b], count[b]);
     if (mass[b]) atomicAdd(&a.mass[(long)n * NB + b], mass[b]);
   }
@@ -226,17 +270,16 @@ __global__ __launch_bounds__(256) void sample_count_kernel(Sample a) {
 // 3. the answers: a block a row
 // ---------------------------------------------------------------------------
 struct Lds {
-  u64 mass[NB];
+  u64 mass[NB];  // running sums, once the row is counted
   unsigned count[NB];
-  union {
-    u64 list[LIST];
-    struct {  // while a bucket is too full for the list
-      u64 mass[NB];
-      unsigned count[NB];
-    } fine;
-  };
-  u64 wave[2][NT / 64];
-  u64 at, before[2], through;
+  u64 list[LIST];
+  // a bucket too full for the list
+  u64 fine_mass[LIST];
+  unsigned fine_count[LIST];
+  double table[STEP];
+  u64 wave[NT / 64];
+  float bound[8];
+  u64 at, through;
   int found;
   unsigned n;
 };
@@ -263,6 +306,19 @@ DEV_INLINE u64 sum_before(u64 v, u64* wave, u64* total) {
   return b + in - v;
 }
 
+// values to their running sums, N = NT * PER of them
+template <int PER, typename V>
+DEV_INLINE void run_sums(V* v, u64* wave) {
+  u64 in[PER], sum = 0, all;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) in[j] = sum += v[threadIdx.x * PER + j];
+  const u64 before = sum_before(sum, wave, &all);
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    v[threadIdx.x * PER + j] = (V)(before + in[j]);
+  __syncthreads();
+}
+
 // a question to the order: its first entry ...
 struct Ask {
   enum Kind {
@@ -278,77 +334,68 @@ DEV_INLINE bool reached(const Ask& q, u64 through) {
                               : (double)through >= q.want;
 }
 
-// The first of NB buckets (two to a thread) with which the question is
-// reached, NB if none, and the weight and number before it.  `weight0` and
-// `number0` lie before all of them.  The first bucket that holds anything may
-// be reached already by what lies before it.
-DEV_INLINE int find_bucket(const Ask& q, const u64* mass,
-                           const unsigned* count, u64 weight0, u64 number0,
-                           Lds& s, u64* weight1, u64* number1) {
-  const int b = threadIdx.x * 2;
-  const bool number = q.kind == Ask::kNumber;
-  const u64 m0 = mass[b], m1 = mass[b + 1];
-  const u64 v0 = number ? count[b] : m0, v1 = number ? count[b + 1] : m1;
-  const u64 base = number ? number0 : weight0;
-  if (threadIdx.x == 0) s.found = NB;
-  u64 all, m = 0;
-  const u64 p0 = base + sum_before(v0 + v1, s.wave[0], &all), p1 = p0 + v0,
-            p2 = p1 + v1;
-  if (number) m = weight0 + sum_before(m0 + m1, s.wave[1], &all);
-  // an empty bucket reaches nothing
-  if (v0 && reached(q, p1) && !(p0 > base && reached(q, p0))) {
-    s.found = b;
-    s.before[0] = number ? m : p0;
-    s.before[1] = p0;
-  } else if (v1 && reached(q, p2) && !(p1 > base && reached(q, p1))) {
-    s.found = b + 1;
-    s.before[0] = number ? m + m0 : p1;
-    s.before[1] = p1;
-  }
-  __syncthreads();
-  const int k = s.found;
-  *weight1 = s.before[0];
-  *number1 = s.before[1];
-  __syncthreads();
-  return k;
+// First of n running sums (behind `base`) with which the question is reached,
+// n if none: each lane looks at one of 64 places, twice.  Every wave does the
+// same search.
+template <typename V>
+DEV_INLINE int find(const Ask& q, const V* sums, int n, u64 base = 0) {
+  const int l = threadIdx.x & 63, step = n / 64;
+  u64 hit = __ballot(reached(q, base + sums[(l + 1) * step - 1]));
+  if (!hit) return n;
+  const int at = (__ffsll((long long)hit) - 1) * step;
+  hit = __ballot(l < step && reached(q, base + sums[at + min(l, step - 1)]));
+  return at + __ffsll((long long)hit) - 1;
 }
 
-// The least logit whose bucket is at most b, by a search in which each lane
-// looks at one of 64 places.  Buckets follow the order, so a bucket is a
-// range of logits, and a scan needs two comparisons for each.
-DEV_INLINE float least_logit(int b, const Row& r) {
-  auto number = [](float v) {
-    const unsigned u = __float_as_uint(v);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-  };
-  auto value = [](unsigned k) {
-    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-  };
+DEV_INLINE int find_bucket(const Ask& q, const Lds& s) {
+  return q.kind == Ask::kNumber ? find(q, s.count, NB) : find(q, s.mass, NB);
+}
+
+template <typename V>
+DEV_INLINE u64 before(const V* sums, int b) { return b ? sums[b - 1] : 0; }
+
+// Float32 and whole numbers in the same order
+DEV_INLINE unsigned rank(float v) {
+  const unsigned u = __float_as_uint(v);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+DEV_INLINE float of_rank(unsigned k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// The rank of the least logit whose bucket is at most b, by a search in which
+// each lane looks at one of 64 places
+DEV_INLINE unsigned least_rank(int b, const Row& r) {
   // the bucket is over b at lo and at most b at hi
-  unsigned lo = number(-kInf), hi = number(r.top);
+  unsigned lo = rank(-kInf), hi = rank(r.ftop);
   while (hi - lo > 1) {
     const unsigned step = (hi - lo + 63) / 64;
     const unsigned at = min(lo + step * ((threadIdx.x & 63) + 1), hi);
-    const int first = __ffsll((unsigned long long)__ballot(
-                          bucket(value(at), r) <= b)) - 1;
-    const unsigned to = min(lo + step * (first + 1), hi);
+    const int first = __ffsll((long long)__ballot(
+                          bucket(depth(of_rank(at), r)) <= b)) - 1;
+    hi = min(lo + step * (first + 1), hi);
     lo += step * first;
-    hi = to;
   }
-  return value(hi);
+  return hi;
 }
 
-// which entries the list holds, so that the next question to the same bucket
-// need not gather them again
-struct Held {
-  int bucket;
-  unsigned n;
-};
+// Buckets follow the order, so buckets (0 to NB - 2) are ranges of logits, and
+// a scan needs two comparisons for each: from low_end on, up to high_end
+DEV_INLINE float low_end(int b, const Row& r) {
+  return of_rank(least_rank(b, r));
+}
+DEV_INLINE float high_end(int b, const Row& r) {
+  return b == 0 ? kInf : of_rank(least_rank(b - 1, r) - 1);
+}
 
 // The list in order: a pair of entries to a thread.  A wave's pairs lie in
 // 128 places of its own while they are at most 64 apart, so only wider steps
 // wait for the other waves.
-DEV_INLINE void sort_list(Lds& s, int size) {
+DEV_INLINE void sort_list(Lds& s, int n) {
+  int size = 2;
+  while (size < n) size <<= 1;
+  for (int i = n + threadIdx.x; i < size; i += NT) s.list[i] = ~0ull;
+  __syncthreads();
   const int i = threadIdx.x;
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
@@ -371,115 +418,142 @@ DEV_INLINE void sort_list(Lds& s, int size) {
   __syncthreads();
 }
 
+// what the list holds, in order: n entries, those of the buckets lo[i] to
+// hi[i] (none where lo > hi) among them all
+struct Held {
+  int lo[3], hi[3];
+  int n;
+};
+
+// Brings the one bucket b to the list; where that cannot hold it (many equal
+// logits), the part of it in which the question is reached, and *weight0 and
+// *number0 then lie before that part.
+template <typename T>
+DEV_INLINE void gather(const Sample& a, const T* x, const Row& r, const Ask& q,
+                       int b, Lds& s, Held* held, u64* weight0,
+                       u64* number0) {
+  const float vlo = low_end(b, r), vhi = high_end(b, r);
+  // entries of the bucket between lo and hi, both included
+  auto each = [&](u64 lo, u64 hi, auto f) {
+    scan_some<T, NT>(
+        x, a.V, [&](float v) { return (v >= vlo) & (v <= vhi); },
+        [&](long i, float v) {
+          const u64 e = entry(v, i);
+          if (e >= lo && e <= hi) f(v, e);
+        });
+  };
+  u64 lo = 0, hi = ~0ull;
+  bool whole_bucket = true;
+  for (;;) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    each(lo, hi, [&](float, u64 e) {
+      const unsigned k = atomicAdd(&s.n, 1u);
+      if (k < LIST) s.list[k] = e;
+    });
+    __syncthreads();
+    if (s.n <= LIST) break;
+    // divide it by the entries' own bits: by 2^10 or more each time
+    whole_bucket = false;
+    u64 least = ~0ull, most = 0;
+    each(lo, hi, [&](float, u64 e) {
+      least = min(least, e);
+      most = max(most, e);
+    });
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      least = min(least, (u64)__shfl_xor(least, off, 64));
+      most = max(most, (u64)__shfl_xor(most, off, 64));
+    }
+    if ((threadIdx.x & 63) == 0) {
+      s.list[threadIdx.x >> 6] = least;
+      s.wave[threadIdx.x >> 6] = most;
+    }
+    for (int i = threadIdx.x; i < LIST; i += NT) {
+      s.fine_mass[i] = 0;
+      s.fine_count[i] = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+      least = min(least, s.list[i]);
+      most = max(most, s.wave[i]);
+    }
+    __syncthreads();
+    // more than LIST = 2^11 different entries: most - least has 12 bits or
+    // 11 of them set, and its 11 highest number the parts
+    const int shift = 53 - (int)__clzll((long long)(most - least));
+    each(least, most, [&](float v, u64 e) {
+      const int k = (int)((e - least) >> shift);
+      atomicAdd(&s.fine_count[k], 1u);
+      const u64 w = weight(depth(v, r), a.sbits, s.table);
+      if (w) atomicAdd(&s.fine_mass[k], w);
+    });
+    __syncthreads();
+    run_sums<LIST / NT>(s.fine_mass, s.wave);
+    run_sums<LIST / NT>(s.fine_count, s.wave);
+    // (the parts' sums are the bucket's, with which the question is reached)
+    const int k = min(LIST - 1, q.kind == Ask::kNumber
+                                    ? find(q, s.fine_count, LIST, *number0)
+                                    : find(q, s.fine_mass, LIST, *weight0));
+    *weight0 += before(s.fine_mass, k);
+    *number0 += before(s.fine_count, k);
+    lo = least + ((u64)k << shift);
+    hi = min(most, lo + ((1ull << shift) - 1));
+  }
+  const int n = (int)s.n;
+  sort_list(s, n);
+  *held = Held{{whole_bucket ? b : 0, 0, 0}, {whole_bucket ? b : -1, -1, -1}, n};
+}
+
 // The question's entry, and the weight through it.  False where it lies in the
 // last bucket or nowhere: the weights there add up to less than 2^-24 of the
 // row's, so no random number below 1 draws them.
 template <typename T>
 DEV_INLINE bool ask(const Sample& a, const T* x, const Row& r, const Ask& q,
-                    Lds& s, Held& held, u64* at, u64* through) {
-  u64 weight0, number0;
-  const int b = find_bucket(q, s.mass, s.count, 0, 0, s, &weight0, &number0);
+                    Lds& s, Held* held, u64* at, u64* through) {
+  const int b = find_bucket(q, s);
   if (b >= NB - 1) return false;
-  if (held.bucket != b) {
-    held.bucket = -1;
-    const float vlo = least_logit(b, r);
-    const float vhi = b ? least_logit(b - 1, r) : kInf;
-    // entries of the bucket between lo and hi, both included
-    auto each = [&](u64 lo, u64 hi, auto f) {
-      scan<T, NT>(x, 0, a.V, [&](long i, float v) {
-        if (!(v >= vlo && (v < vhi || b == 0))) return;
-        const u64 e = entry(v, i);
-        if (e >= lo && e <= hi) f(v, e);
-      });
-    };
-    auto gather = [&](u64 lo, u64 hi) {
-      if (threadIdx.x == 0) s.n = 0;
-      __syncthreads();
-      each(lo, hi, [&](float, u64 e) {
-        const unsigned k = atomicAdd(&s.n, 1u);
-        if (k < LIST) s.list[k] = e;
-      });
-      __syncthreads();
-      return s.n;
-    };
-    u64 lo = 0, hi = ~0ull;
-    unsigned n = gather(lo, hi);
-    const bool whole = n <= LIST;
-    // a bucket that the list cannot hold (many equal logits) is divided by
-    // the entries' own bits until it can: by 2^10 or more each time
-    while (n > LIST) {
-      u64 least = ~0ull, most = 0;
-      each(lo, hi, [&](float, u64 e) {
-        least = min(least, e);
-        most = max(most, e);
-      });
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) {
-        least = min(least, (u64)__shfl_xor(least, off, 64));
-        most = max(most, (u64)__shfl_xor(most, off, 64));
-      }
-      if ((threadIdx.x & 63) == 0) {
-        s.wave[0][threadIdx.x >> 6] = least;
-        s.wave[1][threadIdx.x >> 6] = most;
-      }
-      __syncthreads();  // (and every thread has read s.n)
-      for (int i = threadIdx.x; i < NB; i += NT) {
-        s.fine.mass[i] = 0;
-        s.fine.count[i] = 0;
-      }
-#pragma unroll
-      for (int i = 0; i < NT / 64; ++i) {
-        least = min(least, s.wave[0][i]);
-        most = max(most, s.wave[1][i]);
-      }
-      __syncthreads();
-      // more than LIST different entries: most - least has 11 bits or more
-      const int shift = 53 - (int)__clzll((long long)(most - least));
-      each(least, most, [&](float v, u64 e) {
-        const int k = (int)((e - least) >> shift);
-        atomicAdd(&s.fine.count[k], 1u);
-        const u64 w = weight(depth(v, r), a.sbits);
-        if (w) atomicAdd(&s.fine.mass[k], w);
-      });
-      __syncthreads();
-      const int k = find_bucket(q, s.fine.mass, s.fine.count, weight0,
-                                number0, s, &weight0, &number0);
-      if (k == NB) return false;
-      n = s.fine.count[k];
-      lo = least + ((u64)k << shift);
-      hi = lo + ((1ull << shift) - 1);
-      __syncthreads();
-      if (n <= LIST) n = gather(lo, hi);
-    }
-    int size = 2;
-    while (size < (int)n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += NT) s.list[i] = ~0ull;
-    __syncthreads();
-    sort_list(s, size);
-    // (a part of a bucket is not kept for the next question)
-    held = Held{whole ? b : -1, n};
-  }
-  const int n = (int)held.n, i0 = threadIdx.x * 2;
+  u64 weight0 = before(s.mass, b), number0 = 0;
   const bool number = q.kind == Ask::kNumber;
-  u64 w[2];
+  if (number) number0 = before(s.count, b);
+  bool have = false;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) have |= held->lo[i] <= b && b <= held->hi[i];
+  if (!have) gather(a, x, r, q, b, s, held, &weight0, &number0);
+  // two entries to a thread; the ones of other buckets do not count
+  const int i0 = threadIdx.x * 2;
+  u64 w[2] = {0, 0};
+  unsigned c[2] = {0, 0};
 #pragma unroll
   for (int j = 0; j < 2; ++j)
-    w[j] = i0 + j < n
-               ? weight(depth(entry_logit(s.list[i0 + j]), r), a.sbits) : 0;
+    if (i0 + j < held->n) {
+      const double d = depth(entry_logit(s.list[i0 + j]), r);
+      if (bucket(d) == b) {
+        w[j] = weight(d, a.sbits, s.table);
+        c[j] = 1;
+      }
+    }
   if (threadIdx.x == 0) s.found = LIST;
-  u64 all;
-  const u64 p1 = weight0 + sum_before(w[0] + w[1], s.wave[0], &all) + w[0],
-            p2 = p1 + w[1];
-  const int hit =
-      i0 < n && reached(q, number ? number0 + i0 + 1 : p1)       ? i0
-      : i0 + 1 < n && reached(q, number ? number0 + i0 + 2 : p2) ? i0 + 1
-                                                                 : LIST;
+  u64 all, m = weight0 + sum_before(w[0] + w[1], s.wave, &all);
+  u64 k = number ? number0 + sum_before(c[0] + c[1], s.wave, &all) : 0;
+  int hit = LIST;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    m += w[j];
+    k += c[j];
+    if (hit == LIST && c[j] && reached(q, number ? k : m)) {
+      hit = i0 + j;
+      w[0] = m;  // (taken already)
+    }
+  }
   if (hit < LIST) atomicMin(&s.found, hit);
   __syncthreads();
   const int first = s.found;
   if (first < LIST && first == hit) {
     s.at = s.list[first];
-    s.through = first & 1 ? p2 : p1;
+    s.through = w[0];
   }
   __syncthreads();
   *at = s.at;
@@ -488,31 +562,13 @@ DEV_INLINE bool ask(const Sample& a, const T* x, const Row& r, const Ask& q,
   return first < LIST;
 }
 
-// the weight of the entries that are at most `most` deep
-template <typename T>
-DEV_INLINE u64 shallow(const Sample& a, const T* x, const Row& r, double most,
-                       Lds& s) {
-  // the buckets' bounds are rounded by less than one bucket
-  const int b = max((int)(most * (double)STEP) - 1, 0);
-  u64 v = 0, all;
-  for (int i = threadIdx.x; i < b; i += NT) v += s.mass[i];
-  const float vlo = least_logit(b + 2, r);
-  const float vhi = b ? least_logit(b - 1, r) : kInf;
-  scan<T, NT>(x, 0, a.V, [&](long, float z) {
-    if (!(z >= vlo && (z < vhi || b == 0))) return;
-    const double d = depth(z, r);
-    if (d <= most) v += weight(d, a.sbits);
-  });
-  sum_before(v, s.wave[0], &all);
-  return all;
-}
-
 template <typename T, bool COUNTED>
 __global__ __launch_bounds__(NT) void sample_kernel(Sample a) {
   __shared__ Lds s;
   const int n = blockIdx.x, t = threadIdx.x;
   const T* x = (const T*)a.x + n * a.V;
   float top = -kInf;
+  fill_table(s.table);
   if constexpr (COUNTED) {
     top = parts_top(a, n);
     for (int b = t; b < NB; b += NT) {
@@ -543,34 +599,126 @@ __global__ __launch_bounds__(NT) void sample_kernel(Sample a) {
   const Row r = make_row(temperature(a, n), top);
   const int k = number_kept(a, n, r);
   if constexpr (!COUNTED)
-    count_row<NT>(a, x, 0, a.V, r, k != 0, s.mass, s.count);
+    count_row<NT>(a, x, 0, a.V, r, k != 0, s.table, s.mass, s.count);
   __syncthreads();
+  run_sums<NB / NT>(s.mass, s.wave);
+  if (k) run_sums<NB / NT>(s.count, s.wave);
 
-  Held held = {-1, 0};
-  u64 at = 0, keep, sum, v = 0;
-  for (int b = t; b < NB; b += NT) v += s.mass[b];
-  sum_before(v, s.wave[0], &keep);
-  if (k && ask(a, x, r, Ask{Ask::kNumber, (double)k}, s, held, &at, &sum))
-    keep = sum;
+  // The kept weight lies between keep0 and keep1, as far as whole buckets
+  // say, and so do the buckets of each later question
   const double p = a.pp ? (double)a.pp[n] : a.p;
-  if (p < 1.0 &&
-      ask(a, x, r, Ask{Ask::kWeight, fmax(p, 0.0) * (double)keep}, s, held,
-          &at, &sum))
-    keep = min(keep, sum);
   const double mp = a.mp ? (double)a.mp[n] : a.m;
-  if (mp > 0.0 && !r.greedy) {
-    const double most = fmax(-log(mp), 0.0);
-    if (most * STEP < NB - 4) keep = min(keep, shallow(a, x, r, most, s));
-  }
   const float u = fmaxf(fminf(a.u[n], 1.f - 0x1p-24f), 0.f);
+  u64 keep = s.mass[NB - 1], keep0 = keep, keep1 = keep;
+  Held held = {{0, 0, 0}, {-1, -1, -1}, 0};
+  const Ask ask_k = {Ask::kNumber, (double)k};
+  if (k) {
+    const int b = find_bucket(ask_k, s);
+    if (b < NB - 1) {
+      held.lo[0] = held.hi[0] = b;
+      keep0 = before(s.mass, b);
+      keep1 = s.mass[b];
+    }
+  }
+  const double want_p = fmax(p, 0.0);
+  if (p < 1.0) {
+    const int b0 = find_bucket(Ask{Ask::kWeight, want_p * (double)keep0}, s),
+              b1 = find_bucket(Ask{Ask::kWeight, want_p * (double)keep1}, s);
+    held.lo[1] = b0;
+    held.hi[1] = min(b1, NB - 2);
+    keep0 = min(keep0, before(s.mass, b0));
+    if (b1 < NB) keep1 = min(keep1, s.mass[b1]);
+  }
+  // min_p: whole buckets, and of one the entries that are not too deep
+  const double most = mp > 0.0 ? fmax(-log2(mp) * STEP, 0.0) : 1e9;
+  const bool limit = most < NB - 2 && !r.greedy;
+  const int bm = limit ? bucket(most) : NB;
+  if (limit) {
+    keep0 = min(keep0, before(s.mass, bm));
+    keep1 = min(keep1, s.mass[bm]);
+  }
+  held.lo[2] = find_bucket(Ask{Ask::kOver, (double)u * (double)keep0}, s);
+  held.hi[2] = min(
+      find_bucket(Ask{Ask::kOver, (double)u * (double)keep1}, s), NB - 2);
+
+  // one scan for them all: a wave finds each end of each range
+  if (t < 8 * 64) {
+    const int i = t >> 7, end = t >> 6 & 1;
+    const int lo = i == 0   ? held.lo[0]
+                   : i == 1 ? held.lo[1]
+                   : i == 2 ? held.lo[2]
+                            : bm;
+    const int hi = i == 0   ? held.hi[0]
+                   : i == 1 ? held.hi[1]
+                   : i == 2 ? held.hi[2]
+                            : (limit ? bm : -1);
+    const float v = lo > hi ? __builtin_nanf("")  // no range: holds nothing
+                    : end   ? high_end(lo, r)
+                            : low_end(hi, r);
+    if ((t & 63) == 0) s.bound[t >> 6] = v;
+  }
+  if (t == 0) s.n = 0;
+  __syncthreads();
+  // a range holds what lies within half its width of its middle; the widest
+  // range's half width, a little rounded up, lets all of them through and
+  // little else
+  float vb[8], mid[4], half = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    vb[2 * i] = s.bound[2 * i];
+    vb[2 * i + 1] = fminf(s.bound[2 * i + 1], top);
+    mid[i] = 0.5f * vb[2 * i] + 0.5f * vb[2 * i + 1];
+    half = fmaxf(half, fmaxf(vb[2 * i + 1] - mid[i], mid[i] - vb[2 * i]) *
+                           1.0001f + fabsf(mid[i]) * 1e-6f);
+  }
+  if (top == kInf || !(half < kInf)) {  // no middle of infinite ends
+    half = kInf;
+    mid[0] = 0.f;
+  }
+  u64 part = 0;
+  scan_some<T, NT>(
+      x, a.V,
+      [&](float v) {
+        return fminf(fminf(fabsf(v - mid[0]), fabsf(v - mid[1])),
+                     fminf(fabsf(v - mid[2]), fabsf(v - mid[3]))) <= half;
+      },
+      [&](long i, float v) {
+        if ((v >= vb[0] && v <= vb[1]) || (v >= vb[2] && v <= vb[3]) ||
+            (v >= vb[4] && v <= vb[5])) {
+          const unsigned at = atomicAdd(&s.n, 1u);
+          if (at < LIST) s.list[at] = entry(v, i);
+        }
+        if (v >= vb[6] && v <= vb[7]) {
+          const double d = depth(v, r);
+          if (d <= most) part += weight(d, a.sbits, s.table);
+        }
+      });
+  __syncthreads();
+  held.n = (int)s.n;
+  if (held.n <= LIST)
+    sort_list(s, held.n);
+  else  // too many: each question brings its own
+    held = Held{{0, 0, 0}, {-1, -1, -1}, 0};
+
+  u64 at = 0, sum;
+  if (k && ask(a, x, r, ask_k, s, &held, &at, &sum)) keep = sum;
+  if (p < 1.0 && ask(a, x, r, Ask{Ask::kWeight, want_p * (double)keep}, s,
+                     &held, &at, &sum))
+    keep = min(keep, sum);
+  if (limit) {
+    sum_before(part, s.wave, &sum);
+    keep = min(keep, before(s.mass, bm) + sum);
+  }
   const bool got = ask(a, x, r, Ask{Ask::kOver, (double)u * (double)keep}, s,
-                       held, &at, &sum);
+                       &held, &at, &sum);
   if (t == 0) {
     a.token[n] = got ? (int)(unsigned)at : -1;
-    if (a.logp)
+    if (a.logp) {
+      const float v = entry_logit(at);
+      const double d = v == top ? 0.0 : ((double)top - (double)v) * r.inv;
       a.logp[n] = !got ? __builtin_nanf("")
-                       : (float)(-depth(entry_logit(at), r) -
-                                 log(ldexp((double)keep, -a.sbits)));
+                       : (float)(-d - log(ldexp((double)keep, -a.sbits)));
+    }
   }
 }
 
@@ -581,7 +729,7 @@ void launch(const LaunchCtx& lc, const Sample& a) {
     return;
   }
   sample_max_kernel<T><<<a.N * a.parts, 256, 0, lc.stream>>>(a);
-  sample_count_kernel<T><<<a.N * a.parts, 256, 0, lc.stream>>>(a);
+  sample_count_kernel<T><<<a.N * a.parts, 512, 0, lc.stream>>>(a);
   sample_kernel<T, true><<<a.N, NT, 0, lc.stream>>>(a);
 }
 
@@ -589,7 +737,7 @@ void launch(const LaunchCtx& lc, const Sample& a) {
 // logits; 1 where a block a row is enough
 int parts_of(int64_t N, int64_t V) {
   if (V <= 32768 || N >= 192) return 1;
-  return (int)std::max<int64_t>(1, std::min(1024 / std::max<int64_t>(N, 1),
+  return (int)std::max<int64_t>(1, std::min(512 / std::max<int64_t>(N, 1),
                                             V / 4096));
 }
 
