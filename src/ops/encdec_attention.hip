@@ -234,6 +234,15 @@ DEV_INLINE float pair_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The sequence and key head of the i-th of B * Hk.  Neighbours are sequences,
+// not heads, and go the other way round in every second head: so long and
+// short sequences share each chiplet and each CU.
+DEV_INLINE void seq_head(const Att& a, int i, int* b, int* hk) {
+  *hk = i / a.B;
+  const int k = i - *hk * a.B;
+  *b = *hk & 1 ? a.B - 1 - k : k;
+}
+
 DEV_INLINE int kept_keys(const Att& a, int b) {
   int n = a.Sk;
   if (a.len) n = min(n, max(0, a.len[b]));
@@ -368,12 +377,18 @@ DEV_INLINE void store_part(float* row, const float16_t (&acc)[DP / 32],
 template <typename T, int DP, int KB>
 DEV_INLINE void softmax_step(float16_t (&s)[KB], float16_t (&acc)[DP / 32],
                              float& m, float& l, float c) {
-  float top = kNegInf;
+  // (four chains each for the maximum and the sum: one of 32 dependent
+  // operations would be as long as the products)
+  float t4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
-  top = pair_max(top);
+    for (int i = 0; i < 16; i += 8)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        t4[j] = fmaxf(t4[j], fmaxf(s[kb][i + j], s[kb][i + 4 + j]));
+  const float top =
+      pair_max(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
   // The reference follows the maximum only when that leaves it by more than
   // 2^8: until then the weights are at most 256, which no accumulator
   // minds, and the output is not scaled again
@@ -390,13 +405,15 @@ DEV_INLINE void softmax_step(float16_t (&s)[KB], float16_t (&acc)[DP / 32],
       for (int i = 0; i < 16; ++i) acc[n][i] *= f;
   }
   const float off = m == kNegInf ? 0.f : m * c;
+  float l4[4] = {};
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -off));
-      l += s[kb][i];
+      l4[i & 3] += s[kb][i];
     }
+  l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
 }
 
 // scores of KB blocks of 32 keys, transposed
@@ -490,7 +507,9 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_fwd_kernel(Att
   const int tile = id % mt;
   id /= mt;
   const int split = id % a.nsplit;
-  const int bh = id / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+  int b, hk;
+  seq_head(a, id / a.nsplit, &b, &hk);
+  const int bh = b * a.Hk + hk;
   const int t = threadIdx.x, l = t & 63, h = l >> 5;
   const int row = tile * NW * 32 + (t >> 6) * 32 + (l & 31);
   const bool vec = a.vec;
@@ -544,7 +563,9 @@ __global__ __launch_bounds__(256, (waves<T, DP>(1))) void att_token_kernel(Att a
   const int M = a.G * a.Sq;
   const int id = xcd_swizzle(blockIdx.x, gridDim.x);
   const int split = id % a.nsplit;
-  const int bh = id / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+  int b, hk;
+  seq_head(a, id / a.nsplit, &b, &hk);
+  const int bh = b * a.Hk + hk;
   const int t = threadIdx.x, l = t & 63, h = l >> 5, w = t >> 6;
   const int row = l & 31;
   const bool vec = a.vec;
@@ -667,7 +688,9 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
   const int tile = id % mt;
   id /= mt;
   const int split = id % a.nsplit;
-  const int bh = id / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+  int b, hk;
+  seq_head(a, id / a.nsplit, &b, &hk);
+  const int bh = b * a.Hk + hk;
   const int t = threadIdx.x, l = t & 63, h = l >> 5, r = l & 31;
   const int row = tile * NW * 32 + (t >> 6) * 32 + r;
   const bool vec = a.vec;
@@ -745,7 +768,9 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att
   const int tile = id % kt;
   id /= kt;
   const int split = id % a.nsplit;
-  const int bh = id / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+  int b, hk;
+  seq_head(a, id / a.nsplit, &b, &hk);
+  const int bh = b * a.Hk + hk;
   const int t = threadIdx.x, l = t & 63, h = l >> 5, r = l & 31;
   const int k0 = tile * NW * 32 + (t >> 6) * 32, key = k0 + r;
   const bool vec = a.vec;
