@@ -254,15 +254,31 @@ DEV_INLINE int kept_keys(const Att& a, int b) {
 // Every load is done, from a row that exists, and what is not wanted (a row
 // past the end, a masked key, columns from D on) becomes zeros on its way to
 // LDS: loads under a condition would be waited for where the branch ends, and
-// a NaN in a masked key's memory meets no product.
+// a NaN in a masked key's memory meets no product.  Most tiles are whole, and
+// their rows lie at one distance: those need no arithmetic at all, a scalar
+// base for each load and one offset a thread.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int ROWS, int NT>
 struct Stage {
   using TL = Tile<T, DP>;
   static constexpr int N = ROWS * TL::CPR / NT;
-  static_assert(ROWS * TL::CPR % NT == 0, "whole chunks a thread");
+  static constexpr int STEP = NT / TL::CPR;  // rows between a thread's chunks
+  static_assert(ROWS * TL::CPR % NT == 0 && NT % TL::CPR == 0,
+                "whole chunks and rows");
   int4_t r[N];
   unsigned want;  // a bit a chunk
+  // the thread's offset in bytes, for rows `ss` elements apart
+  static DEV_INLINE unsigned offset(int t, long ss, int D) {
+    const int d = t % TL::CPR * TL::EPC;
+    return (unsigned)((t / TL::CPR * ss + (d < D ? d : 0)) * sizeof(T));
+  }
+  // all rows from `base` on
+  DEV_INLINE void load(const T* base, long ss, unsigned off, int t, int D) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      r[i] = *(const int4_t*)((const char*)(base + i * STEP * ss) + off);
+    want = t % TL::CPR * TL::EPC < D ? ~0u : 0;
+  }
   // ptr(i): the i-th row, or another that exists; ok(i): whether it is wanted
   template <typename P, typename K>
   DEV_INLINE void load(P ptr, K ok, int t, int D, bool vec) {
@@ -270,28 +286,32 @@ struct Stage {
     if (vec) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int row = (i * NT + t) / TL::CPR;
-        const int d = (i * NT + t) % TL::CPR * TL::EPC;
+        const int row = i * STEP + t / TL::CPR, d = t % TL::CPR * TL::EPC;
         r[i] = *(const int4_t*)(ptr(row) + (d < D ? d : 0));
         if (d < D && ok(row)) want |= 1u << i;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int row = (i * NT + t) / TL::CPR;
-        r[i] = load_chunk<T>(ptr(row), (i * NT + t) % TL::CPR * TL::EPC, D,
-                             false);
+        const int row = i * STEP + t / TL::CPR;
+        r[i] = load_chunk<T>(ptr(row), t % TL::CPR * TL::EPC, D, false);
         if (ok(row)) want |= 1u << i;
       }
     }
   }
-  DEV_INLINE void store(char* tile, int t) const {
+  // `all`: every chunk is wanted
+  DEV_INLINE void store(char* tile, int t, bool all) const {
+    if (all) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = i * NT + t;
-      const int4_t zero = {0, 0, 0, 0};
-      *(int4_t*)(tile + TL::at(c / TL::CPR, c % TL::CPR)) =
-          want >> i & 1 ? r[i] : zero;
+      for (int i = 0; i < N; ++i)
+        *(int4_t*)(tile + TL::at(i * STEP + t / TL::CPR, t % TL::CPR)) = r[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int4_t zero = {0, 0, 0, 0};
+        *(int4_t*)(tile + TL::at(i * STEP + t / TL::CPR, t % TL::CPR)) =
+            want >> i & 1 ? r[i] : zero;
+      }
     }
   }
 };
@@ -300,37 +320,58 @@ struct Stage {
 // ones whose mask is not 0
 template <typename T, int DP, int BN, int NT>
 struct KeyTiles {
-  Stage<T, DP, BN, NT> k, v;
+  using S = Stage<T, DP, BN, NT>;
+  S k, v;
   const T *kb, *vb;
   long ks, vs;
   const uint8_t* mask;
-  int n;
-  DEV_INLINE KeyTiles(const Att& a, int b, int hk, int kept)
+  int n, D, t;
+  unsigned ko, vo;
+  bool vec;
+  DEV_INLINE KeyTiles(const Att& a, int b, int hk, int kept, int thread)
       : kb(row_ptr<T>(a.k, b, hk, 0)), vb(row_ptr<T>(a.v, b, hk, 0)),
         ks(a.k.ss), vs(a.v.ss),
-        mask(a.mask ? a.mask + (long)b * a.Sk : nullptr), n(kept) {}
+        mask(a.mask ? a.mask + (long)b * a.Sk : nullptr), n(kept), D(a.D),
+        t(thread), ko(S::offset(thread, a.k.ss, a.D)),
+        vo(S::offset(thread, a.v.ss, a.D)), vec(a.vec) {}
   DEV_INLINE bool ok(int key) const {
     return key < n && (!mask || mask[min(key, n - 1)]);
   }
-  DEV_INLINE void load(int tile, int t, int D, bool vec) {
+  // whether a tile has keys that are left out
+  DEV_INLINE bool partial(int tile) const {
+    return mask || (tile + 1) * BN > n;
+  }
+  DEV_INLINE void load(int tile) {
     const int k0 = tile * BN;
+    if (vec && !partial(tile)) {
+      k.load(kb + k0 * ks, ks, ko, t, D);
+      v.load(vb + k0 * vs, vs, vo, t, D);
+      return;
+    }
     auto good = [&](int r) { return ok(k0 + r); };
     k.load([&](int r) { return kb + min(k0 + r, n - 1) * ks; }, good, t, D,
            vec);
     v.load([&](int r) { return vb + min(k0 + r, n - 1) * vs; }, good, t, D,
            vec);
   }
-  DEV_INLINE void store(char* lk, char* lv, uint8_t* keep, int tile,
-                        int t) const {
-    k.store(lk, t);
-    v.store(lv, t);
-    for (int r = t; r < BN; r += NT) keep[r] = ok(tile * BN + r);
-  }
-  // whether a tile has keys that are left out
-  DEV_INLINE bool partial(int tile) const {
-    return mask || (tile + 1) * BN > n;
+  DEV_INLINE void store(char* lk, char* lv, uint8_t* keep, int tile) const {
+    const bool all = D == DP && !partial(tile);
+    k.store(lk, t, all);
+    v.store(lv, t, all);
+    if (partial(tile))
+      for (int r = t; r < BN; r += NT) keep[r] = ok(tile * BN + r);
   }
 };
+
+// f(0), f(1), ... for i in [t0, t1), with the buffer's number as a constant:
+// addresses in LDS then differ by constants only
+template <typename F>
+DEV_INLINE void in_turn(int t0, int t1, F f) {
+  for (int i = t0; i < t1; i += 2) {
+    f(i, std::integral_constant<int, 0>{});
+    if (i + 1 < t1) f(i + 1, std::integral_constant<int, 1>{});
+  }
+}
 
 // O^T (or dQ^T) accumulators of one row per lane pair to memory
 template <typename T, int DP>
@@ -386,7 +427,7 @@ DEV_INLINE void softmax_step(float16_t (&s)[KB], float16_t (&acc)[DP / 32],
     for (int i = 0; i < 16; i += 8)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        t4[j] = fmaxf(t4[j], fmaxf(s[kb][i + j], s[kb][i + 4 + j]));
+        t4[j] = fmaxf(fmaxf(t4[j], s[kb][i + j]), s[kb][i + 4 + j]);
   const float top =
       pair_max(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
   // The reference follows the maximum only when that leaves it by more than
@@ -526,23 +567,24 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_fwd_kernel(Att
   float16_t acc[DP / 32] = {};
   float m = kNegInf, sum = 0.f;
 
-  KeyTiles<T, DP, BN, NT> kt(a, b, hk, n);
+  KeyTiles<T, DP, BN, NT> kt(a, b, hk, n, t);
   if (t0 < t1) {
-    kt.load(t0, t, a.D, vec);
-    kt.store(lk[0], lv[0], lkeep[0], t0, t);
+    kt.load(t0);
+    kt.store(lk[0], lv[0], lkeep[0], t0);
   }
   __syncthreads();
-  for (int i = t0; i < t1; ++i) {
-    const int buf = (i - t0) & 1;
-    if (i + 1 < t1) kt.load(i + 1, t, a.D, vec);
+  in_turn(t0, t1, [&](int i, auto number) __attribute__((always_inline)) {
+    constexpr int buf = decltype(number)::value;
+    if (i + 1 < t1) kt.load(i + 1);
     float16_t s[KB];
     scores<T, DP, KB>(lk[buf], qf, s, l);
     if (kt.partial(i)) drop_keys<KB>(lkeep[buf], s, h);
     softmax_step<T, DP, KB>(s, acc, m, sum, a.scale * kLog2e);
     weigh<T, DP, KB>(lv[buf], s, acc, l);
-    if (i + 1 < t1) kt.store(lk[buf ^ 1], lv[buf ^ 1], lkeep[buf ^ 1], i + 1, t);
+    if (i + 1 < t1)
+      kt.store(lk[buf ^ 1], lv[buf ^ 1], lkeep[buf ^ 1], i + 1);
     __syncthreads();
-  }
+  });
   sum = pair_sum(sum);
   finish_row<T, DP>(a, acc, m, sum, split, b, hk, row, h);
 }
@@ -583,16 +625,16 @@ __global__ __launch_bounds__(256, (waves<T, DP>(1))) void att_token_kernel(Att a
   float m = kNegInf, sum = 0.f;
   char *lk = lds[w], *lv = lds[w] + BYTES;
 
-  KeyTiles<T, DP, BN, 64> kt(a, b, hk, n);
-  if (t0 < t1) kt.load(t0, l, a.D, vec);
+  KeyTiles<T, DP, BN, 64> kt(a, b, hk, n, l);
+  if (t0 < t1) kt.load(t0);
   for (int i = t0; i < t1; ++i) {
-    kt.store(lk, lv, lkeep[w], i, l);
+    kt.store(lk, lv, lkeep[w], i);
     // a wave's LDS accesses are done in order; the fence keeps the compiler
     // from moving the reads of other lanes' values over these writes
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (i + 1 < t1) kt.load(i + 1, l, a.D, vec);
+    if (i + 1 < t1) kt.load(i + 1);
     float16_t s[KB];
     scores<T, DP, KB>(lk, qf, s, l);
     if (kt.partial(i)) drop_keys<KB>(lkeep[w], s, h);
@@ -725,15 +767,15 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
   }
   float16_t acc[DP / 32] = {};
 
-  KeyTiles<T, DP, BN, NT> kt(a, b, hk, n);
+  KeyTiles<T, DP, BN, NT> kt(a, b, hk, n, t);
   if (t0 < t1) {
-    kt.load(t0, t, a.D, vec);
-    kt.store(lk[0], lv[0], lkeep[0], t0, t);
+    kt.load(t0);
+    kt.store(lk[0], lv[0], lkeep[0], t0);
   }
   __syncthreads();
-  for (int i = t0; i < t1; ++i) {
-    const int buf = (i - t0) & 1;
-    if (i + 1 < t1) kt.load(i + 1, t, a.D, vec);
+  in_turn(t0, t1, [&](int i, auto number) __attribute__((always_inline)) {
+    constexpr int buf = decltype(number)::value;
+    if (i + 1 < t1) kt.load(i + 1);
     float16_t s[KB], dp[KB];
     scores<T, DP, KB>(lk[buf], qf, s, l);
     scores<T, DP, KB>(lv[buf], gf, dp, l);
@@ -745,9 +787,10 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
         s[kb][j] = __builtin_amdgcn_exp2f(fmaf(s[kb][j], c, -lse)) *
                    (dp[kb][j] - delta);
     weigh<T, DP, KB>(lk[buf], s, acc, l);
-    if (i + 1 < t1) kt.store(lk[buf ^ 1], lv[buf ^ 1], lkeep[buf ^ 1], i + 1, t);
+    if (i + 1 < t1)
+      kt.store(lk[buf ^ 1], lv[buf ^ 1], lkeep[buf ^ 1], i + 1);
     __syncthreads();
-  }
+  });
   if (row >= M) return;
   if (a.nsplit > 1)
     store_part<DP>(a.part + part_row(a, split, bh, row) * DP, acc, h);
@@ -792,24 +835,38 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att
   }
   float16_t dk[DP / 32] = {}, dv[DP / 32] = {};
 
-  Stage<T, DP, BM, NT> sq, sg;
-  auto fetch = [&](int i) {
-    auto ok = [&](int rr) { return i * BM + rr < M; };
+  using S = Stage<T, DP, BM, NT>;
+  S sq, sg;
+  const unsigned qo = S::offset(t, a.q.ss, a.D),
+                 go = S::offset(t, a.dout.ss, a.D);
+  float rl = 0.f, rd = 0.f;  // one row's log-sum and dO . O
+  static_assert(BM <= NT, "a row a thread");
+  auto fetch = [&](int i) __attribute__((always_inline)) {
+    const int m0 = i * BM, g = m0 / a.Sq, s0 = m0 - g * a.Sq;
+    const long at = (long)bh * M + min(m0 + t, M - 1);
+    rl = a.lse[at];
+    rd = a.delta[at];
+    if (vec && s0 + BM <= a.Sq) {  // rows of one head
+      sq.load(row_ptr<T>(a.q, b, hk * a.G + g, s0), a.q.ss, qo, t, a.D);
+      sg.load(row_ptr<T>(a.dout, b, hk * a.G + g, s0), a.dout.ss, go, t, a.D);
+      return;
+    }
+    auto ok = [&](int rr) { return m0 + rr < M; };
     sq.load([&](int rr) -> const T* {
-      return q_row<T>(a.q, a, b, hk, min(i * BM + rr, M - 1));
+      return q_row<T>(a.q, a, b, hk, min(m0 + rr, M - 1));
     }, ok, t, a.D, vec);
     sg.load([&](int rr) -> const T* {
-      return q_row<T>(a.dout, a, b, hk, min(i * BM + rr, M - 1));
+      return q_row<T>(a.dout, a, b, hk, min(m0 + rr, M - 1));
     }, ok, t, a.D, vec);
   };
-  auto put = [&](int i, int buf) {
-    sq.store(lq[buf], t);
-    sg.store(lg[buf], t);
-    for (int k = t; k < BM; k += NT) {
-      const int m = i * BM + k;
+  auto put = [&](int i, int buf) __attribute__((always_inline)) {
+    const bool all = a.D == DP && (i + 1) * BM <= M;
+    sq.store(lq[buf], t, all);
+    sg.store(lg[buf], t, all);
+    if (t < BM) {
       // a row past the end has a weight of exp2(-inf)
-      llse[buf][k] = m < M ? a.lse[(long)bh * M + m] : -kNegInf;
-      ldel[buf][k] = m < M ? a.delta[(long)bh * M + m] : 0.f;
+      llse[buf][t] = i * BM + t < M ? rl : -kNegInf;
+      ldel[buf][t] = i * BM + t < M ? rd : 0.f;
     }
   };
   if (t0 < t1) {
@@ -817,8 +874,8 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att
     put(t0, 0);
   }
   __syncthreads();
-  for (int i = t0; i < t1; ++i) {
-    const int buf = (i - t0) & 1;
+  in_turn(t0, t1, [&](int i, auto number) __attribute__((always_inline)) {
+    constexpr int buf = decltype(number)::value;
     if (i + 1 < t1) fetch(i + 1);
 #pragma unroll
     for (int mb = 0; mb < BM / 32; ++mb) {
@@ -857,7 +914,7 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att
     }
     if (i + 1 < t1) put(i + 1, buf ^ 1);
     __syncthreads();
-  }
+  });
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -1016,7 +1073,9 @@ Att make_att(const Arr& q, const Arr& kv, const Arr& values, int heads,
 bool vectors(std::initializer_list<View> vs, int D, size_t size) {
   if ((D * size) % 16) return false;  // then so are all strides
   for (auto& v : vs)
-    if ((uintptr_t)v.p & 15) return false;
+    // (a tile's rows are offsets of 32 bits from its first)
+    if (((uintptr_t)v.p & 15) || v.ss * 64 * (long)size >= 1L << 31)
+      return false;
   return true;
 }
 
