@@ -199,7 +199,7 @@ def _encdec_sizes(q, kv, heads, kv_heads, tnc):
     B = q.shape[0]
     if tnc:
         B, sq, sk = q.shape[1], q.shape[0], kv.shape[0]
-    return B, heads, kv_heads, sq, sk, q.shape[2] // heads
+    return B, heads, kv_heads, sq, sk, q.shape[2] // heads, _FLAG[q.dtype]
 
 
 def _encdec_work(sizes, which, device):

@@ -449,7 +449,8 @@ bool _registered = [] {
       const auto ins = Arrs(in);
       const EncDec e = ReadEncDec(a, ins.data(), ins.size());
       const int64_t n = encdec_attention_workspace(e.B, e.heads, e.kv_heads,
-                                                   e.sq, e.sk, e.D)[0];
+                                                   e.sq, e.sk, e.D,
+                                                   e.q.dtype)[0];
       encdec_attention_fwd_raw(LC(o), e.q, e.kv, e.values, e.heads,
                                e.kv_heads, e.len, e.mask, e.tnc, out[0],
                                out[1], Scratch(o, n, kFloat32));
@@ -477,7 +478,8 @@ bool _registered = [] {
       const auto ins = Arrs(in, 3);
       const EncDec e = ReadEncDec(a, ins.data(), ins.size());
       const int64_t n = encdec_attention_workspace(e.B, e.heads, e.kv_heads,
-                                                   e.sq, e.sk, e.D)[1];
+                                                   e.sq, e.sk, e.D,
+                                                   e.q.dtype)[1];
       encdec_attention_bwd_raw(LC(o), in[0], e.q, e.kv, e.values, e.heads,
                                e.kv_heads, e.len, e.mask, e.tnc, in[1], in[2],
                                out[0], out[1],

@@ -272,11 +272,15 @@ struct Stage {
     const int d = t % TL::CPR * TL::EPC;
     return (unsigned)((t / TL::CPR * ss + (d < D ? d : 0)) * sizeof(T));
   }
-  // all rows from `base` on
+  // all rows from `base` on; `once`: nobody reads them again
+  template <bool once = false>
   DEV_INLINE void load(const T* base, long ss, unsigned off, int t, int D) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      r[i] = *(const int4_t*)((const char*)(base + i * STEP * ss) + off);
+    for (int i = 0; i < N; ++i) {
+      const int4_t* p =
+          (const int4_t*)((const char*)(base + i * STEP * ss) + off);
+      r[i] = once ? __builtin_nontemporal_load(p) : *p;
+    }
     want = t % TL::CPR * TL::EPC < D ? ~0u : 0;
   }
   // ptr(i): the i-th row, or another that exists; ok(i): whether it is wanted
@@ -318,7 +322,7 @@ struct Stage {
 
 // the keys and values of one tile; `n` keys are kept (n >= 1), of those the
 // ones whose mask is not 0
-template <typename T, int DP, int BN, int NT>
+template <typename T, int DP, int BN, int NT, bool once = false>
 struct KeyTiles {
   using S = Stage<T, DP, BN, NT>;
   S k, v;
@@ -344,8 +348,8 @@ struct KeyTiles {
   DEV_INLINE void load(int tile) {
     const int k0 = tile * BN;
     if (vec && !partial(tile)) {
-      k.load(kb + k0 * ks, ks, ko, t, D);
-      v.load(vb + k0 * vs, vs, vo, t, D);
+      k.template load<once>(kb + k0 * ks, ks, ko, t, D);
+      v.template load<once>(vb + k0 * vs, vs, vo, t, D);
       return;
     }
     auto good = [&](int r) { return ok(k0 + r); };
@@ -590,8 +594,7 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_fwd_kernel(Att
 }
 
 // ---------------------------------------------------------------------------
-// forward of at most 32 rows (single tokens): each of 4 waves takes its own
-// keys, in its own part of LDS and without a barrier; the waves' results are
+// forward of at most 32 rows (single tokens): each wave takes its own keys, in its own part of LDS and without a barrier; the waves' results are
 // joined at the end.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int BN>
@@ -625,7 +628,7 @@ __global__ __launch_bounds__(256, (waves<T, DP>(1))) void att_token_kernel(Att a
   float m = kNegInf, sum = 0.f;
   char *lk = lds[w], *lv = lds[w] + BYTES;
 
-  KeyTiles<T, DP, BN, 64> kt(a, b, hk, n, l);
+  KeyTiles<T, DP, BN, 64, true> kt(a, b, hk, n, l);
   if (t0 < t1) kt.load(t0);
   for (int i = t0; i < t1; ++i) {
     kt.store(lk, lv, lkeep[w], i);
@@ -683,31 +686,35 @@ __global__ __launch_bounds__(256, (waves<T, DP>(1))) void att_token_kernel(Att a
   finish_row<T, DP>(a, acc, top, sum, split, b, hk, row, h);
 }
 
-// joins the splits of the forward: a wave a row
+// joins the splits of the forward: a wave a row.  Lane k has the k-th split's
+// maximum and sum (there are at most 64), so only the values are read in turn,
+// and no read waits for another.
 template <typename T>
 __global__ __launch_bounds__(256) void att_join_kernel(Att a, int DP) {
   const int M = a.G * a.Sq, l = threadIdx.x & 63;
   const long rows = (long)a.B * a.Hk * M;
   const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (at >= rows) return;
-  const float* ml = a.part + (long)a.nsplit * rows * DP;
+  const float* ml = a.part + (long)a.nsplit * rows * DP +
+                    ((long)min(l, a.nsplit - 1) * rows + at) * 2;
   const float c = a.scale * kLog2e;
-  float top = kNegInf;
-  for (int k = 0; k < a.nsplit; ++k)
-    top = fmaxf(top, ml[(k * rows + at) * 2]);
-  float sum = 0.f, o0 = 0.f, o1 = 0.f;
+  const float m = l < a.nsplit ? ml[0] : kNegInf;
+  const float top = wave_reduce_max(m);
+  const float f =
+      m == kNegInf ? 0.f : __builtin_amdgcn_exp2f((m - top) * c);
+  const float sum = wave_reduce_sum(m == kNegInf ? 0.f : ml[1] * f);
+  float o0 = 0.f, o1 = 0.f;
+  const float* o = a.part + at * DP + min(l, DP - 1);
+  const float* p = a.part + at * DP + min(l + 64, DP - 1);
+#pragma unroll 4
   for (int k = 0; k < a.nsplit; ++k) {
-    const float m = ml[(k * rows + at) * 2];
-    if (m == kNegInf) continue;
-    const float f = __builtin_amdgcn_exp2f((m - top) * c);
-    const float* o = a.part + (k * rows + at) * DP;
-    sum += ml[(k * rows + at) * 2 + 1] * f;
-    if (l < DP) o0 += o[l] * f;
-    if (l + 64 < DP) o1 += o[l + 64] * f;
+    const float fk = __shfl(f, k, 64);
+    // (a split without a key wrote zeros)
+    o0 += o[k * rows * DP] * fk;
+    if (DP > 64) o1 += p[k * rows * DP] * fk;
   }
   const long bh = at / M;
-  const int m = (int)(at - bh * M);
-  T* out = q_row<T>(a.o, a, bh / a.Hk, (int)(bh % a.Hk), m);
+  T* out = q_row<T>(a.o, a, bh / a.Hk, (int)(bh % a.Hk), (int)(at - bh * M));
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   if (l < a.D) out[l] = (T)(o0 * inv);
   if (l + 64 < a.D) out[l + 64] = (T)(o1 * inv);
@@ -977,11 +984,10 @@ __global__ __launch_bounds__(256) void att_dkv_join_kernel(Att a, int DP) {
 // ---------------------------------------------------------------------------
 int pad_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// as many splits as bring the launch to about two blocks a CU, but none
-// shorter than `least` tiles
-int splits(long blocks, long tiles, long least) {
-  long n = std::min(512 / std::max<long>(blocks, 1),
-                    tiles / std::max<long>(least, 1));
+// As many splits as bring the launch to `want` blocks, none shorter than
+// `least` tiles of 64
+int splits(long blocks, long want, long tiles, long least) {
+  const long n = std::min(want / std::max<long>(blocks, 1), tiles / least);
   return (int)std::max<long>(1, std::min<long>(n, 64));
 }
 
@@ -989,19 +995,27 @@ struct Plan {
   int DP, NW, fwd, dq, dkv, kw;  // waves of rows, splits, waves of keys
 };
 
-// NW = 0: the kernel for single tokens
-Plan make_plan(long B, long H, long Hk, long Sq, long Sk, long D) {
+// NW = 0: the kernel for single tokens.
+// Two blocks a CU (512) are wanted: twice that, to even out sequences of
+// different lengths, gained nothing (one token of 8x32 heads over 8192 to
+// 16384 keys: 87 us to 85).
+// A split costs a launch and its partial results, so it has four tiles (about
+// 4 us) or more; one tile in fp32, whose products take 16 times as long.
+Plan make_plan(long B, long H, long Hk, long Sq, long Sk, long D, int dtype) {
   Plan p;
   const long M = H / Hk * Sq, bh = B * Hk;
+  const long least = dtype == kFloat32 ? 1 : 4;
   p.DP = pad_dim((int)D);
   p.NW = M <= 32 ? 0 : M <= 64 ? 2 : 4;
   const int rows = std::max(p.NW, 1) * 32;
   const long tiles = (Sk + 63) / 64;
-  p.fwd = splits(bh * ((M + rows - 1) / rows), tiles, p.NW ? 4 : 8);
+  p.fwd = splits(bh * ((M + rows - 1) / rows), 512, tiles,
+                 p.NW ? least : 8);
   const int qrows = p.NW == 4 ? 128 : 64;
-  p.dq = splits(bh * ((M + qrows - 1) / qrows), tiles, 4);
+  p.dq = splits(bh * ((M + qrows - 1) / qrows), 512, tiles, least);
   p.kw = Sk <= 64 ? 2 : 4;
-  p.dkv = splits(bh * ((Sk + p.kw * 32 - 1) / (p.kw * 32)), (M + 63) / 64, 4);
+  p.dkv = splits(bh * ((Sk + p.kw * 32 - 1) / (p.kw * 32)), 512,
+                 (M + 63) / 64, least);
   return p;
 }
 
@@ -1108,7 +1122,9 @@ void fwd(const LaunchCtx& lc, Att a, const Plan& p) {
     const unsigned n = grid(bh * a.nsplit *
                             (p.NW ? (M + p.NW * 32 - 1) / (p.NW * 32) : 1));
     if (p.NW == 0)
-      // a wave's own tile of 16 KB at most
+      // a wave's own tile of 16 KB at most.  (Tiles of 32 keys in blocks of
+      // eight waves, four a SIMD: 21 us for 32x16 heads over 512 keys of 64,
+      // where this takes 17.)
       att_token_kernel<T, DP, sizeof(T) == 2 && DP <= 64 ? 64 : 32>
           <<<n, 256, 0, lc.stream>>>(a);
     else if (p.NW == 2)
@@ -1164,10 +1180,11 @@ int64_t align4(int64_t n) { return (n + 3) & ~(int64_t)3; }
 
 std::vector<int64_t> encdec_attention_workspace(int64_t B, int64_t H,
                                                 int64_t Hk, int64_t Sq,
-                                                int64_t Sk, int64_t D) {
+                                                int64_t Sk, int64_t D,
+                                                int dtype) {
   MX_CHECK(H > 0 && Hk > 0 && H % Hk == 0 && D > 0,
            "encdec_attention: bad heads");
-  const Plan p = make_plan(B, H, Hk, Sq, Sk, D);
+  const Plan p = make_plan(B, H, Hk, Sq, Sk, D, dtype);
   const int64_t rows = B * H * Sq;
   const int64_t fwd = p.fwd > 1 ? p.fwd * rows * (p.DP + 2) : 0;
   const int64_t dq = p.dq > 1 ? p.dq * rows * p.DP : 0;
@@ -1183,15 +1200,15 @@ void encdec_attention_fwd_raw(const LaunchCtx& lc, const Arr& q,
                               const Arr& work) {
   if (out.numel() == 0) return;
   Att a = make_att(q, kv, values, heads, kv_heads, len, mask, tnc);
-  const Plan p = make_plan(a.B, a.H, a.Hk, a.Sq, a.Sk, a.D);
+  const Plan p = make_plan(a.B, a.H, a.Hk, a.Sq, a.Sk, a.D, q.dtype);
   MX_CHECK(out.shape == q.shape && out.dtype == q.dtype,
            "encdec_attention: the output must be like the queries");
   MX_CHECK(!lse.defined() ||
                (lse.dtype == kFloat32 && lse.numel() == (long)a.B * a.H * a.Sq),
            "encdec_attention: one float32 for each row of each head");
   MX_CHECK((work.defined() && work.dtype == kFloat32 ? work.numel() : 0) >=
-               encdec_attention_workspace(a.B, a.H, a.Hk, a.Sq, a.Sk,
-                                          a.D)[0],
+               encdec_attention_workspace(a.B, a.H, a.Hk, a.Sq, a.Sk, a.D,
+                                          q.dtype)[0],
            "encdec_attention: workspace too small");
   a.o = view(out, lead(out, tnc, "out"), 0, a.D);
   a.lse = lse.data<float>();
@@ -1209,7 +1226,7 @@ void encdec_attention_bwd_raw(const LaunchCtx& lc, const Arr& dout,
                               const Arr& dvalues, const Arr& work) {
   if (dkv.numel() == 0 && dq.numel() == 0) return;
   Att a = make_att(q, kv, values, heads, kv_heads, len, mask, tnc);
-  const Plan p = make_plan(a.B, a.H, a.Hk, a.Sq, a.Sk, a.D);
+  const Plan p = make_plan(a.B, a.H, a.Hk, a.Sq, a.Sk, a.D, q.dtype);
   MX_CHECK(dout.shape == q.shape && dout.dtype == q.dtype &&
                out.shape == q.shape && out.dtype == q.dtype &&
                dq.shape == q.shape && dq.dtype == q.dtype &&
@@ -1222,8 +1239,8 @@ void encdec_attention_bwd_raw(const LaunchCtx& lc, const Arr& dout,
   MX_CHECK(rows == 0 || (lse.dtype == kFloat32 && lse.numel() == rows),
            "encdec_attention backward: one float32 for each row");
   MX_CHECK((work.defined() && work.dtype == kFloat32 ? work.numel() : 0) >=
-               encdec_attention_workspace(a.B, a.H, a.Hk, a.Sq, a.Sk,
-                                          a.D)[1],
+               encdec_attention_workspace(a.B, a.H, a.Hk, a.Sq, a.Sk, a.D,
+                                          q.dtype)[1],
            "encdec_attention backward: workspace too small");
   a.o = view(out, lead(out, tnc, "out"), 0, a.D);
   a.dout = view(dout, lead(dout, tnc, "dout"), 0, a.D);

@@ -90,7 +90,8 @@ void rms_norm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
 // encdec_attention_workspace gives, {forward, backward}
 std::vector<int64_t> encdec_attention_workspace(int64_t B, int64_t H,
                                                 int64_t Hk, int64_t Sq,
-                                                int64_t Sk, int64_t D);
+                                                int64_t Sk, int64_t D,
+                                                int dtype);
 void encdec_attention_fwd_raw(const LaunchCtx& lc, const Arr& q,
                               const Arr& kv, const Arr& values, int heads,
                               int kv_heads, const Arr& len, const Arr& mask,
