@@ -178,10 +178,14 @@ def encdec_attention(queries, keys_values, values=None, heads=1,
             valid_length = valid_length.to(torch.int32).contiguous()
         if mask is not None:
             mask = mask.contiguous()
-        return _EncDecAttention.apply(
-            q.contiguous(), kv.contiguous(),
-            None if values is None else values.contiguous(), valid_length,
-            mask, heads, kv_heads, tnc)
+        q, kv = q.contiguous(), kv.contiguous()
+        values = None if values is None else values.contiguous()
+        if not _nn.needs_grad(q, kv, values):
+            return hip_required('encdec_attention').encdec_attention_fwd(
+                q, kv, values, heads, kv_heads, valid_length, mask, tnc,
+                False)[0]
+        return _EncDecAttention.apply(q, kv, values, valid_length, mask,
+                                      heads, kv_heads, tnc)
     if tnc:
         q, kv = q.transpose(0, 1), kv.transpose(0, 1)
         values = None if values is None else values.transpose(0, 1)

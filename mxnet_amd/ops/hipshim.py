@@ -28,8 +28,17 @@ def _arr(t):
 
 
 def _dev_stream(t):
-    dev = t.device.index or 0
-    return dev, torch.cuda.current_stream(dev).cuda_stream
+    dev = t.get_device()
+    return dev, _raw_stream(dev)
+
+
+def _raw_stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+if hasattr(torch._C, '_cuda_getCurrentRawStream'):
+    # the same handle without a Stream object (1 us a call)
+    _raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811
 
 
 def _c(t):
@@ -449,15 +458,16 @@ def layernorm_bwd(dy, x, gamma, mean, istd):
     return [dx, dgamma.to(gamma.dtype), dbeta.to(gamma.dtype)]
 
 
-def rms_norm_fwd(x, gamma, residual, eps, int8=False):
+def rms_norm_fwd(x, gamma, residual, eps, int8=False, want_stat=True):
     """(y, sum or None, rstd), or with int8 (q, sum or None, scale); the
-    statistic keeps the leading axes, with a last one of 1."""
+    statistic keeps the leading axes, with a last one of 1 (None without
+    want_stat, where no backward follows)."""
     x = _c(x)
     dev, s = _dev_stream(x)
     y = torch.empty(x.shape, dtype=torch.int8 if int8 else x.dtype,
                     device=x.device)
     stat = torch.empty(x.shape[:-1] + (1,), dtype=torch.float32,
-                       device=x.device)
+                       device=x.device) if want_stat else None
     res = _c(residual) if residual is not None else None
     total = torch.empty_like(x) if res is not None else None
     st = _arr(stat)

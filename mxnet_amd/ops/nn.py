@@ -617,6 +617,12 @@ class _RMSNorm(torch.autograd.Function):
         return dx, dgamma, dx if ctx.needs_input_grad[2] else None, None
 
 
+def needs_grad(*tensors):
+    """Whether autograd has to see an operator of these (or None)."""
+    return torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in tensors)
+
+
 def _rms_norm_check(x, gamma, residual, out_type):
     if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise TypeError(f'RMSNorm: float16, bfloat16 or float32 data, got '
@@ -650,9 +656,7 @@ def rms_norm(x, gamma, residual=None, axis=-1, eps=1e-6, out_type=None):
         raise NotImplementedError('rms_norm only over the last axis')
     _rms_norm_check(x, gamma, residual, out_type)
     if out_type == 'int8':
-        if torch.is_grad_enabled() and any(
-                t is not None and t.requires_grad
-                for t in (x, gamma, residual)):
+        if needs_grad(x, gamma, residual):
             raise ValueError('RMSNorm: the int8 output has no gradient; call '
                              'it outside autograd.record() or on detached '
                              'arrays')
@@ -661,6 +665,10 @@ def rms_norm(x, gamma, residual=None, axis=-1, eps=1e-6, out_type=None):
                 x, gamma, residual, eps, int8=True)
             return (q, scale) if h is None else (q, scale, h)
     elif use_hip(x) and x.numel():
+        if not needs_grad(x, gamma, residual):
+            y, h, _ = hip_required('rms_norm').rms_norm_fwd(
+                x, gamma, residual, eps, want_stat=False)
+            return y if residual is None else (y, h)
         return _RMSNorm.apply(x.contiguous(), gamma,
                               None if residual is None
                               else residual.contiguous(), eps)

@@ -461,15 +461,15 @@ DEV_INLINE void softmax_step(float16_t (&s)[KB], float16_t (&acc)[DP / 32],
   l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
 }
 
-// scores of KB blocks of 32 keys, transposed
+// scores of KB blocks of 32 keys, transposed, added to `from`
 template <typename T, int DP, int KB>
 DEV_INLINE void scores(const char* kt,
                        const typename Mat<T>::Frag (&qf)[DP / 16],
-                       float16_t (&s)[KB], int l) {
+                       float16_t (&s)[KB], int l, float16_t from) {
   const int r = l & 31, h = l >> 5;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    s[kb] = float16_t{};
+    s[kb] = from;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks)
       s[kb] = Mat<T>::mma(Tile<T, DP>::row_frag(kt, kb * 32 + r, ks, h),
@@ -581,7 +581,7 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_fwd_kernel(Att
     constexpr int buf = decltype(number)::value;
     if (i + 1 < t1) kt.load(i + 1);
     float16_t s[KB];
-    scores<T, DP, KB>(lk[buf], qf, s, l);
+    scores<T, DP, KB>(lk[buf], qf, s, l, float16_t{});
     if (kt.partial(i)) drop_keys<KB>(lkeep[buf], s, h);
     softmax_step<T, DP, KB>(s, acc, m, sum, a.scale * kLog2e);
     weigh<T, DP, KB>(lv[buf], s, acc, l);
@@ -639,7 +639,7 @@ __global__ __launch_bounds__(256, (waves<T, DP>(1))) void att_token_kernel(Att a
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     if (i + 1 < t1) kt.load(i + 1);
     float16_t s[KB];
-    scores<T, DP, KB>(lk, qf, s, l);
+    scores<T, DP, KB>(lk, qf, s, l, float16_t{});
     if (kt.partial(i)) drop_keys<KB>(lkeep[w], s, h);
     softmax_step<T, DP, KB>(s, acc, m, sum, a.scale * kLog2e);
     weigh<T, DP, KB>(lv, s, acc, l);
@@ -772,7 +772,10 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
     if (split == 0 && h == 0 && row < M)
       a.delta[(long)bh * M + row] = delta;
   }
-  float16_t acc[DP / 32] = {};
+  // dP is added to -delta by its products
+  float16_t acc[DP / 32] = {}, less;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) less[j] = -delta;
 
   KeyTiles<T, DP, BN, NT> kt(a, b, hk, n, t);
   if (t0 < t1) {
@@ -784,15 +787,15 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
     constexpr int buf = decltype(number)::value;
     if (i + 1 < t1) kt.load(i + 1);
     float16_t s[KB], dp[KB];
-    scores<T, DP, KB>(lk[buf], qf, s, l);
-    scores<T, DP, KB>(lv[buf], gf, dp, l);
+    scores<T, DP, KB>(lk[buf], qf, s, l, float16_t{});
+    scores<T, DP, KB>(lv[buf], gf, dp, l, less);
     if (kt.partial(i)) drop_keys<KB>(lkeep[buf], s, h);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        s[kb][j] = __builtin_amdgcn_exp2f(fmaf(s[kb][j], c, -lse)) *
-                   (dp[kb][j] - delta);
+        s[kb][j] =
+            __builtin_amdgcn_exp2f(fmaf(s[kb][j], c, -lse)) * dp[kb][j];
     weigh<T, DP, KB>(lk[buf], s, acc, l);
     if (i + 1 < t1)
       kt.store(lk[buf ^ 1], lv[buf ^ 1], lkeep[buf ^ 1], i + 1);
@@ -873,7 +876,7 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att
     if (t < BM) {
       // a row past the end has a weight of exp2(-inf)
       llse[buf][t] = i * BM + t < M ? rl : -kNegInf;
-      ldel[buf][t] = i * BM + t < M ? rd : 0.f;
+      ldel[buf][t] = i * BM + t < M ? -rd : 0.f;
     }
   };
   if (t0 < t1) {
@@ -886,7 +889,15 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att
     if (i + 1 < t1) fetch(i + 1);
 #pragma unroll
     for (int mb = 0; mb < BM / 32; ++mb) {
-      float16_t s = {}, dp = {};
+      // dP is added to -delta by its products
+      float16_t s = {}, dp;
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const float4_t less =
+            *(const float4_t*)&ldel[buf][mb * 32 + 2 * j + 4 * h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[j + e] = less[e];
+      }
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks)
         s = Mat<T>::mma(TL::row_frag(lq[buf], mb * 32 + r, ks, h), kf[ks], s);
@@ -898,13 +909,10 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att
       for (int j = 0; j < 16; j += 4) {
         const int at = mb * 32 + 2 * j + 4 * h;
         const float4_t lse = *(const float4_t*)&llse[buf][at];
-        const float4_t del = *(const float4_t*)&ldel[buf][at];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[j + e], c, -lse[e]));
-          p = keep ? p : 0.f;
-          s[j + e] = p;
-          dp[j + e] = p * (dp[j + e] - del[e]);
+          s[j + e] = __builtin_amdgcn_exp2f(fmaf(s[j + e], c, -lse[e]));
+          dp[j + e] *= s[j + e];
         }
       }
 #pragma unroll
@@ -922,12 +930,16 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att
     if (i + 1 < t1) put(i + 1, buf ^ 1);
     __syncthreads();
   });
+  // a key that is not kept had weights too (its scores were zeros), which went
+  // to its own row alone and become zeros here
+  const unsigned kept = (unsigned)__ballot(keep);
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const int k = k0 + 8 * (j / 4) + 4 * h + (j & 3), col = d * 32 + r;
       if (k >= a.Sk) continue;
+      if (!(kept >> (k - k0) & 1)) dk[d][j] = dv[d][j] = 0.f;
       if (a.nsplit > 1) {
         float* p = a.part +
                    (((long)split * a.B * a.Hk + bh) * a.Sk + k) * 2 * DP;

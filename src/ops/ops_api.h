@@ -73,7 +73,8 @@ void layernorm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& x,
 
 // ---- rmsnorm.hip ----------------------------------------------------------
 // h = x (+ residual, written to sum); y = h * rstd * gamma, or int8 with one
-// scale a row where y's dtype is int8 (then rstd is not written)
+// scale a row where y's dtype is int8 (then rstd is not written; it may be
+// undefined where no backward follows)
 void rms_norm_fwd_raw(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
                       const Arr& residual, double eps, const Arr& y,
                       const Arr& scale, const Arr& sum, const Arr& rstd);

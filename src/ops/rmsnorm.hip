@@ -145,7 +145,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
   }
   s = row_sum<TPR>(s, red);
   const float r = inv_rms(s, C, eps);
-  if (!INT8 && lane == 0) rstd[row] = r;
+  if (!INT8 && rstd && lane == 0) rstd[row] = r;
   if constexpr (!INT8) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(1024) void rms_fwd_long_kernel(
     }
     s = row_sum<1024>(s, red);
     const float r = inv_rms(s, C, eps);
-    if (!INT8 && threadIdx.x == 0) rstd[row] = r;
+    if (!INT8 && rstd && threadIdx.x == 0) rstd[row] = r;
     float sc = 0.f, inv = 0.f;
     if constexpr (INT8) {
       float a = 0.f;
@@ -523,7 +523,8 @@ void rms_norm_fwd_raw(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
                     sum.numel() == x.numel() && sum.dtype == x.dtype),
            "RMSNorm: the residual and the sum must be like the data");
   const Arr& stat = int8 ? scale : rstd;
-  MX_CHECK(stat.defined() && stat.dtype == kFloat32 && stat.numel() == rows,
+  MX_CHECK(stat.defined() ? stat.dtype == kFloat32 && stat.numel() == rows
+                          : !int8,
            "RMSNorm: one float32 value a row is needed beside the output");
   DISPATCH_FLOAT_NATIVE(x.dtype, "RMSNorm", [&] {
     auto go = [&](auto r, auto q) {
