@@ -234,19 +234,31 @@ DEV_INLINE float pair_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The sequence and key head of the i-th of B * Hk.  Neighbours are sequences,
-// not heads, and go the other way round in every second head: so long and
-// short sequences share each chiplet and each CU.
-DEV_INLINE void seq_head(const Att& a, int i, int* b, int* hk) {
-  *hk = i / a.B;
-  const int k = i - *hk * a.B;
-  *b = *hk & 1 ? a.B - 1 - k : k;
-}
-
 DEV_INLINE int kept_keys(const Att& a, int b) {
   int n = a.Sk;
   if (a.len) n = min(n, max(0, a.len[b]));
   return n;
+}
+
+// The sequence and key head of the i-th of B * Hk.  Neighbours are sequences,
+// not heads, the longest first, and the shortest first in every second head:
+// so each chiplet has work of every length, a CU's two blocks are a long and a
+// short one where all blocks run at once, and where they do not the short ones
+// come last.  A wave sorts up to 64 lengths by counting.
+DEV_INLINE void seq_head(const Att& a, int i, int* b, int* hk) {
+  *hk = i / a.B;
+  int k = i - *hk * a.B;
+  if (*hk & 1) k = a.B - 1 - k;
+  *b = k;
+  if (!a.len || a.B > 64) return;
+  const int l = threadIdx.x & 63;
+  const int n = l < a.B ? kept_keys(a, l) : -1;
+  int place = 0;
+  for (int j = 0; j < a.B; ++j) {
+    const int m = __builtin_amdgcn_readlane(n, j);
+    place += m > n || (m == n && j < l);
+  }
+  *b = __ffsll((long long)__ballot(l < a.B && place == k)) - 1;
 }
 
 // ---------------------------------------------------------------------------
