@@ -1129,12 +1129,11 @@ void by_dim(int DP, F f) {
   else f(std::integral_constant<int, 128>{});
 }
 
-// rows a tile of `n` operands in registers: 64, or 32 where those, the tile on
-// its way and the accumulators would not fit the registers of two waves
+// Rows a tile: 64 where two waves' registers hold it on its way beside their
+// operands and accumulators, else 32 (forward of 4x16 heads, 1024 over 2048
+// keys of 128 in bf16: 100 us with 32, 115 with 64, which spills)
 template <typename T, int DP>
-constexpr int tile_rows(int n) {
-  return n * DP * (int)sizeof(T) <= 256 && sizeof(T) == 2 ? 64 : 32;
-}
+constexpr int tile_rows() { return sizeof(T) == 2 && DP <= 64 ? 64 : 32; }
 
 template <typename T>
 void fwd(const LaunchCtx& lc, Att a, const Plan& p) {
@@ -1142,7 +1141,7 @@ void fwd(const LaunchCtx& lc, Att a, const Plan& p) {
   a.nsplit = p.fwd;
   const long bh = (long)a.B * a.Hk, M = (long)a.G * a.Sq;
   by_dim(p.DP, [&](auto dp) {
-    constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>(1);
+    constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>();
     const unsigned n = grid(bh * a.nsplit *
                             (p.NW ? (M + p.NW * 32 - 1) / (p.NW * 32) : 1));
     if (p.NW == 0)
@@ -1167,7 +1166,7 @@ void bwd(const LaunchCtx& lc, Att a, const Plan& p) {
   if (M) {
     a.nsplit = p.dq;
     by_dim(p.DP, [&](auto dp) {
-      constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>(2);
+      constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>();
       if (p.NW == 4)
         att_dq_kernel<T, DP, 4, BN>
             <<<grid(bh * a.nsplit * ((M + 127) / 128)), 256, 0, lc.stream>>>(
@@ -1183,7 +1182,7 @@ void bwd(const LaunchCtx& lc, Att a, const Plan& p) {
   if (a.Sk) {
     a.nsplit = p.dkv;
     by_dim(p.DP, [&](auto dp) {
-      constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>(2);
+      constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>();
       const int keys = p.kw * 32;
       const unsigned n = grid(bh * a.nsplit * ((a.Sk + keys - 1) / keys));
       if (p.kw == 4)

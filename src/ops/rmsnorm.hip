@@ -358,24 +358,27 @@ __global__ __launch_bounds__(256) void rms_dgamma_long_kernel(
   partial[(long)blockIdx.y * C + c] = v;
 }
 
-// dgamma[c] = sum of the partials' column c: 64 columns a block, 16 threads a
-// column, always in the same order
+// dgamma[c] = sum of the partials' column c: 32 columns a block, 32 threads a
+// column, eight reads of each on their way, always in the same order
 __global__ __launch_bounds__(1024) void rms_dgamma_kernel(
     const float* __restrict__ partial, float* __restrict__ dgamma, int nblk,
     int C) {
-  __shared__ float part[16][64];
-  const int col = threadIdx.x & 63, k = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + col;
+  __shared__ float part[32][33];
+  const int col = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + col;
   float v = 0.f;
-  if (c < C)
-    for (int b = k; b < nblk; b += 16) v += partial[(long)b * C + c];
+  if (c < C) {
+#pragma unroll 8
+    for (int b = k; b < nblk; b += 32) v += partial[(long)b * C + c];
+  }
   part[k][col] = v;
   __syncthreads();
-  if (k == 0 && c < C) {
+  // a wave takes two columns: 32 lanes add one
+  const int mine = threadIdx.x >> 5, from = threadIdx.x & 31;
+  v = part[from][mine];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += part[i][col];
-    dgamma[c] = v;
-  }
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if (from == 0 && blockIdx.x * 32 + mine < C) dgamma[blockIdx.x * 32 + mine] = v;
 }
 
 // ---------------------------------------------------------------------------
@@ -569,7 +572,7 @@ void rms_norm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
       bwd_launch<scalar_t, false>(lc, dy, dsum, h, gamma, rstd, dx,
                                   partial.data<float>(), (int)nblk);
   });
-  rms_dgamma_kernel<<<(unsigned)((C + 63) / 64), 1024, 0, lc.stream>>>(
+  rms_dgamma_kernel<<<(unsigned)((C + 31) / 32), 1024, 0, lc.stream>>>(
       partial.data<float>(), dgamma.data<float>(), rows ? (int)nblk : 0,
       (int)C);
   HIP_CHECK_LAST();
