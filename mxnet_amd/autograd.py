@@ -107,6 +107,17 @@ def mark_variables(variables, gradients, grad_reqs='write'):
         v._t.grad = g._t
 
 
+def _engine_threads(tensors):
+    """Context for torch's backward pass.  Of heads on one GPU it runs in the
+    calling thread: handing each pass to the device's thread and waiting for
+    it costs about 50 us, and no second device could work meanwhile.  Heads
+    on several devices keep a thread for each."""
+    one = tensors and tensors[0].is_cuda and all(
+        t.device == tensors[0].device for t in tensors)
+    return torch.autograd.set_multithreading_enabled(
+        not one and torch._C._is_multithreading_enabled())
+
+
 def backward(heads, head_grads=None, retain_graph=False, train_mode=True):
     """Compute gradients of heads w.r.t. marked variables.
 
@@ -136,7 +147,8 @@ def backward(heads, head_grads=None, retain_graph=False, train_mode=True):
             head_grads = [head_grads]
         grads = [g._t if g is not None else torch.ones_like(t)
                  for g, t in zip(head_grads, tensors)]
-    torch.autograd.backward(tensors, grads, retain_graph=retain_graph)
+    with _engine_threads(tensors):
+        torch.autograd.backward(tensors, grads, retain_graph=retain_graph)
 
 
 def grad(heads, variables, head_grads=None, retain_graph=None,
@@ -152,9 +164,10 @@ def grad(heads, variables, head_grads=None, retain_graph=None,
         if isinstance(head_grads, NDArray):
             head_grads = [head_grads]
         gr = [g._t for g in head_grads]
-    outs = torch.autograd.grad(tensors, [v._t for v in variables], gr,
-                               retain_graph=retain_graph,
-                               create_graph=create_graph)
+    with _engine_threads(tensors):
+        outs = torch.autograd.grad(tensors, [v._t for v in variables], gr,
+                                   retain_graph=retain_graph,
+                                   create_graph=create_graph)
     return [NDArray(o) for o in outs]
 
 
