@@ -197,7 +197,7 @@ def RMSNorm(data, gamma, residual=None, axis=-1, eps=1e-6, out_type=None,
     through both.  With ``out_type='int8'`` (inference) y is given as
     ``q * scale``, int8 values and one float32 scale a row, for an int8
     product: ``[q, scale]`` or ``[q, scale, h]``.  A row of zeros has a scale
-    of 1; a row that holds a NaN or an infinity has one of NaN.
+    of 1; a row whose norm holds a NaN or an infinity has one of NaN.
     """
     if data.is_native:
         if axis not in (-1, data.ndim - 1):

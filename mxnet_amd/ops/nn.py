@@ -686,8 +686,8 @@ def rms_norm(x, gamma, residual=None, axis=-1, eps=1e-6, out_type=None):
     some = (top > 0) & ~torch.isinf(inv)
     scale = torch.where(some, top * (1.0 / 127.0), torch.ones_like(top))
     q = torch.round(y * torch.where(some, inv, torch.zeros_like(top)))
-    # a row with a NaN or an infinity has no scale
-    bad = ~torch.isfinite(hf).all(-1, keepdim=True)
+    # a row whose norm is not finite everywhere has no scale
+    bad = ~torch.isfinite(y).all(-1, keepdim=True)
     scale = scale.masked_fill(bad, float('nan'))
     q = q.masked_fill(bad, 0.0).clamp(-127, 127).to(torch.int8)
     return (q, scale) if residual is None else (q, scale, h)

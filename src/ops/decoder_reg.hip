@@ -101,15 +101,18 @@ void RmsCpu(const NodeAttrs& a, const OpCtx&, V in, V out) {
       continue;
     }
     float top = 0.f;
-    for (long c = 0; c < C; ++c)
-      top = std::max(top, std::fabs(h[c] * inv * g[c]));
+    bool bad = false;
+    for (long c = 0; c < C; ++c) {
+      const float y = std::fabs(h[c] * inv * g[c]);
+      bad |= !std::isfinite(y);
+      top = std::max(top, y);
+    }
     float f = 127.0f * (1.0f / top);
     *stat = top * (1.0f / 127.0f);
     if (!(top > 0.f) || std::isinf(f)) {
       *stat = 1.f;
       f = 0.f;
     }
-    const bool bad = !std::isfinite(sq);
     if (bad) *stat = std::numeric_limits<float>::quiet_NaN();
     for (long c = 0; c < C; ++c) {
       const float q = bad ? 0.f : std::nearbyint(h[c] * inv * g[c] * f);

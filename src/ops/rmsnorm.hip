@@ -62,13 +62,14 @@ DEV_INLINE float row_sum_f32(float v, float* red) {
 }
 
 template <int TPR>
-DEV_INLINE float row_max(float v, float* red) {
-  v = wave_reduce_max(v);
+DEV_INLINE unsigned row_max(unsigned v, unsigned* red) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
   if constexpr (TPR > 64) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < TPR / 64; ++i) v = fmaxf(v, red[i]);
+    for (int i = 0; i < TPR / 64; ++i) v = max(v, red[i]);
     __syncthreads();
   }
   return v;
@@ -78,17 +79,25 @@ DEV_INLINE float inv_rms(double sumsq, int C, double eps) {
   return (float)(1.0 / sqrt(sumsq / C + eps));
 }
 
+// The largest magnitude is taken of the values' bits, which order infinities
+// and NaN (of the row, or that gamma made) above all numbers.
+constexpr unsigned kInfBits = 0x7f800000u;
+DEV_INLINE unsigned magnitude(float v) {
+  return __float_as_uint(v) & 0x7fffffffu;
+}
+
 // a row's scale and its reciprocal.  A row of zeros (or so small that
-// 127 / a overflows) quantises to zeros under a scale of 1; a row that holds
-// a NaN or an infinity has a sum that is not finite, and a scale of NaN.
-DEV_INLINE void int8_scale(float a, double sumsq, float* scale, float* inv) {
+// 127 / a overflows) quantises to zeros under a scale of 1; a row whose norm
+// is not finite everywhere, to zeros under a scale of NaN.
+DEV_INLINE void int8_scale(unsigned bits, float* scale, float* inv) {
+  const float a = __uint_as_float(bits);
   *scale = a * (1.0f / 127.0f);
   *inv = 127.0f * (1.0f / a);
-  if (!(a > 0.f) || isinf(*inv)) {
+  if (bits == 0 || isinf(*inv)) {
     *scale = 1.f;
     *inv = 0.f;
   }
-  if (!isfinite(sumsq)) {
+  if (bits >= kInfBits) {
     *scale = __builtin_nanf("");
     *inv = 0.f;
   }
@@ -160,7 +169,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
     }
   } else {
     float v[NV][VEC];
-    float a = 0.f;
+    unsigned a = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
@@ -169,13 +178,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           v[i][j] = (float)h[i][j] * r * g[j];
-          a = fmaxf(a, fabsf(v[i][j]));
+          a = max(a, magnitude(v[i][j]));
         }
       }
     }
-    a = row_max<TPR>(a, (float*)red);
+    a = row_max<TPR>(a, (unsigned*)red);
     float sc, inv;
-    int8_scale(a, s, &sc, &inv);
+    int8_scale(a, &sc, &inv);
     if (lane == 0) scale[row] = sc;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -216,11 +225,11 @@ __global__ __launch_bounds__(1024) void rms_fwd_long_kernel(
     if (!INT8 && rstd && threadIdx.x == 0) rstd[row] = r;
     float sc = 0.f, inv = 0.f;
     if constexpr (INT8) {
-      float a = 0.f;
+      unsigned a = 0;
       for (int c = threadIdx.x; c < C; c += 1024)
-        a = fmaxf(a, fabsf(value(c) * r * gamma[c]));
-      a = row_max<1024>(a, (float*)red);
-      int8_scale(a, s, &sc, &inv);
+        a = max(a, magnitude(value(c) * r * gamma[c]));
+      a = row_max<1024>(a, (unsigned*)red);
+      int8_scale(a, &sc, &inv);
       if (threadIdx.x == 0) scale[row] = sc;
     }
     for (int c = threadIdx.x; c < C; c += 1024) {

@@ -321,3 +321,14 @@ def test_int8_product_behind_the_norm():
     wd = w.double() * 0.01
     off = 0.5 * s.to_torch().double() * wd.abs().sum(1)[None]
     assert ((out.double() - y @ wd.T).abs() <= off * 1.01).all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_int8_of_a_gamma_that_is_not_finite(native, device):
+    x = np.random.RandomState(11).randn(3, 40).astype('float32')
+    for value in (np.nan, np.inf):
+        g = np.ones(40, 'float32')
+        g[7] = value
+        q, scale = mx.nd.RMSNorm(arr(x, device), arr(g, device),
+                                 out_type='int8')
+        assert np.isnan(scale.asnumpy()).all() and not q.asnumpy().any()

@@ -305,3 +305,16 @@ def test_gluon_layer_and_symbol(tmp_path):
     assert torch.equal(got[0].to_torch(), y2.to_torch())
     assert torch.equal(mx.sym.RMSNorm(a, g, eps=1e-5).eval_dict(feed)[0]
                        .to_torch(), y.to_torch())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('cols', [64, 1001, 33000])
+@pytest.mark.parametrize('value', [float('nan'), float('inf')])
+def test_int8_of_a_gamma_that_is_not_finite(value, cols, device):
+    """No row can be scaled then: a finite scale would hide the value."""
+    x = torch.randn(3, cols, device=device)
+    gamma = torch.ones(cols, device=device)
+    gamma[cols // 2] = value
+    q, scale = mx.nd.RMSNorm(mx.nd.from_torch(x), mx.nd.from_torch(gamma),
+                             out_type='int8')
+    assert torch.isnan(scale.to_torch()).all() and not q.to_torch().any()
