@@ -608,6 +608,7 @@ class _RMSNorm(torch.autograd.Function):
         return y if residual is None else (y, total)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dsum=None):
         h, gamma, rstd = ctx.saved_tensors
         if dy is None:  # only the sum was used

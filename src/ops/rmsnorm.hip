@@ -495,13 +495,21 @@ void fwd_launch(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
                                    sum.ptr}));
   T* yp = INT8 ? nullptr : (T*)y.ptr;
   signed char* qp = INT8 ? (signed char*)y.ptr : nullptr;
+  // a launch has fewer than 2^32 threads: 2^21 blocks of 1024 at most
 #define LAUNCH()                                                            \
   constexpr int RPB = TPR < 256 ? 256 / TPR : 1;                            \
-  rms_fwd_kernel<T, VEC, TPR, NV, RES, INT8>                                \
-      <<<(unsigned)((rows + RPB - 1) / RPB), TPR < 256 ? 256 : TPR, 0,      \
-         lc.stream>>>(x.data<T>(), res.data<T>(), gamma.data<float>(), yp,  \
-                      qp, scale.data<float>(), sum.data<T>(),               \
-                      rstd.data<float>(), rows, C, eps)
+  for (long r0 = 0; r0 < rows; r0 += (1L << 21) * RPB) {                    \
+    const long n = std::min(rows - r0, (1L << 21) * RPB), at = r0 * C;      \
+    rms_fwd_kernel<T, VEC, TPR, NV, RES, INT8>                              \
+        <<<(unsigned)((n + RPB - 1) / RPB), TPR < 256 ? 256 : TPR, 0,       \
+           lc.stream>>>(                                                    \
+            x.data<T>() + at, RES ? res.data<T>() + at : nullptr,           \
+            gamma.data<float>(), INT8 ? nullptr : yp + at,                  \
+            INT8 ? qp + at : nullptr,                                       \
+            INT8 ? scale.data<float>() + r0 : nullptr,                      \
+            RES ? sum.data<T>() + at : nullptr,                             \
+            rstd.defined() ? rstd.data<float>() + r0 : nullptr, n, C, eps); \
+  }
   RMS_DISPATCH((int)(16 / sizeof(T)))
 #undef LAUNCH
   rms_fwd_long_kernel<T, RES, INT8>

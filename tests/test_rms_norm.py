@@ -318,3 +318,65 @@ def test_int8_of_a_gamma_that_is_not_finite(value, cols, device):
     q, scale = mx.nd.RMSNorm(mx.nd.from_torch(x), mx.nd.from_torch(gamma),
                              out_type='int8')
     assert torch.isnan(scale.to_torch()).all() and not q.to_torch().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('out_type', [None, 'int8'])
+def test_more_rows_than_one_launch_takes(out_type):
+    """2^32 threads or more are not one launch: 2^23 rows of a wave each."""
+    x = torch.randn((1 << 23) + 5, 1, device='cuda:0').half()
+    res = torch.randn((1 << 23) + 5, 1, device='cuda:0').half()
+    gamma = torch.full((1,), 0.75, device='cuda:0')
+    out = mx.nd.RMSNorm(mx.nd.from_torch(x), mx.nd.from_torch(gamma),
+                        residual=mx.nd.from_torch(res), out_type=out_type)
+    h, r, want = oracle(x, gamma, res)
+    assert torch.equal(out[-1].to_torch(), h)
+    if out_type is None:
+        rel, least = half_step(torch.float16)
+        within(out[0].to_torch(), want,
+               want.abs() * (rel * (1 + 8 * U32) + 4 * U32) + least)
+    else:
+        y = h.float() * r.float() * gamma
+        q, scale = out[0].to_torch(), out[1].to_torch()
+        assert torch.equal(q, 127 * torch.sign(y).to(torch.int8))
+        some = torch.where(y == 0, 1.0, y.abs() * (1.0 / 127.0))
+        assert torch.equal(scale, some)
+
+
+@pytest.mark.gpu
+def test_past_2_31_elements():
+    """The last rows of 4 GB give what they give alone, forward and back."""
+    rows, cols = (1 << 19) + 6, 4096
+    d = make(6, cols, torch.bfloat16, 'cuda:0', seed=5)
+    big = torch.zeros(rows, cols, dtype=torch.bfloat16, device='cuda:0')
+    dy = torch.zeros_like(big)
+    big[-6:], dy[-6:] = d['x'], d['dy']
+    both = []
+    for x, g in ((d['x'], d['dy']), (big, dy)):
+        x, gamma = (mx.nd.from_torch(t.detach().requires_grad_())
+                    for t in (x, d['gamma']))
+        with autograd.record():
+            y = mx.nd.RMSNorm(x, gamma)
+        dx, dg = autograd.grad([y], [x, gamma], [mx.nd.from_torch(g)])
+        both.append((y.to_torch()[-6:].detach().clone(),
+                     dx.to_torch()[-6:].clone(), dg.to_torch()))
+    (y0, dx0, dg0), (y1, dx1, dg1) = both
+    # (few rows take a block each, many a wave: other orders of 32-bit sums)
+    rel, least = half_step(torch.bfloat16)
+    assert torch.equal(y0, y1)
+    for a, b, scale in ((dx0, dx1, 1.0), (dg0, dg1, 0.0)):
+        a, b = a.double(), b.double()
+        size = a.abs().amax()
+        within(a, b, a.abs() * 2 * rel * scale + size * cols * 4 * U32 + least)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    d = make(4, 64, torch.float32, 'cuda:0', seed=6)
+    x = d['x'].requires_grad_()
+    with autograd.record():
+        y = mx.nd.RMSNorm(mx.nd.from_torch(x), mx.nd.from_torch(d['gamma']))
+    dx, = autograd.grad([y], [mx.nd.from_torch(x)], create_graph=True,
+                        retain_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.to_torch().square().sum().backward()
