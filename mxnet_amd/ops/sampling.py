@@ -24,6 +24,8 @@ def _param(name, value, n, device, dtype, low, high):
                              f'{value.device}')
         if value.is_floating_point() != dtype.is_floating_point:
             raise TypeError(f'sample_tokens: {name} of {value.dtype}')
+        if value.dtype == torch.int64:  # int32 may not hold it
+            value = value.clamp(0, high)
         return value.to(dtype).contiguous()
     return check_number(name, value, str(dtype).replace('torch.', ''), low,
                         high)

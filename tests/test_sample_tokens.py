@@ -229,3 +229,26 @@ def test_refusals():
             (TypeError, x, u, dict(top_p=nd(torch.ones(2).int())))]:
         with pytest.raises(error):
             f(nd(a), nd(b), **kw)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_top_k_that_int32_does_not_hold(device):
+    x, u = make(3, 50, torch.float32, device, seed=12)
+    k = torch.tensor([(1 << 32) + 1, 1 << 31, 2], device=device)
+    check(x, u, top_k=k)
+
+
+@pytest.mark.gpu
+def test_past_2_31_logits():
+    """The last rows of 4 GB draw what they draw alone."""
+    n, v = 8200, (1 << 18) + 8
+    x = torch.empty(n, v, dtype=torch.float16, device='cuda:0')
+    for i in range(0, n, 1000):
+        x[i:i + 1000].normal_()
+    u = torch.rand(n, device='cuda:0')
+    last = x[-3:].clone()
+    kw = dict(temperature=0.8, top_k=200, top_p=0.9, get_prob=True)
+    token, logp = mx.nd.contrib.sample_tokens(nd(x), nd(u), **kw)
+    alone = mx.nd.contrib.sample_tokens(nd(last), nd(u[-3:].clone()), **kw)
+    assert torch.equal(token.to_torch()[-3:], alone[0].to_torch())
+    assert torch.equal(logp.to_torch()[-3:], alone[1].to_torch())
