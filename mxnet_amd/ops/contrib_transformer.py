@@ -91,6 +91,7 @@ class _EncDecAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, kv, values, length, mask, out, lse = ctx.saved_tensors
         heads, kv_heads, tnc = ctx.conf
@@ -175,6 +176,8 @@ def encdec_attention(queries, keys_values, values=None, heads=1,
     _encdec_check(q, kv, values, heads, kv_heads, valid_length, mask, tnc)
     if use_hip(q):
         if valid_length is not None:
+            if valid_length.dtype != torch.int32:  # which may not hold all
+                valid_length = valid_length.clamp(0, kv.shape[0 if tnc else 1])
             valid_length = valid_length.to(torch.int32).contiguous()
         if mask is not None:
             mask = mask.contiguous()

@@ -1081,9 +1081,11 @@ Att make_att(const Arr& q, const Arr& kv, const Arr& values, int heads,
   MX_CHECK(!mask.defined() || ((mask.dtype == kUint8 || mask.dtype == kBool) &&
                                mask.numel() == hk.B * hk.S),
            name << ": the mask must hold one byte for each key");
+  // (the quotient of a row by Sq comes from a reciprocal in float32, at most
+  // one off for up to 2^20 heads)
   MX_CHECK(hq.S * heads < (1L << 30) && hk.S < (1L << 30) &&
-               hq.B * heads < (1L << 30),
-           name << ": too many rows, keys or sequences");
+               hq.B * heads < (1L << 30) && heads <= (1 << 20),
+           name << ": too many rows, keys, heads or sequences");
   Att a = {};
   a.q = view(q, hq, 0, D);
   if (values.defined()) {
@@ -1117,8 +1119,9 @@ bool vectors(std::initializer_list<View> vs, int D, size_t size) {
   return true;
 }
 
+// (a launch has fewer than 2^32 threads: 2^24 blocks of 256)
 unsigned grid(long blocks) {
-  MX_CHECK(blocks < (1L << 31), "encdec_attention: too many blocks");
+  MX_CHECK(blocks < (1L << 24), "encdec_attention: too many sequences");
   return (unsigned)blocks;
 }
 

@@ -335,3 +335,79 @@ def test_refusals_on_the_gpu():
         mx.nd.contrib.encdec_attention(nd(q), nd(q), nd(q), heads=1)
     with pytest.raises(ValueError):
         mx.nd.contrib.encdec_attention(nd(q), nd(q.cpu()), nd(q), heads=2)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_lengths_that_int32_does_not_hold(device):
+    size = (3, 2, 1, 2, 9, 8)
+    far = [(1 << 32) + 2, -(1 << 40), 1 << 31]
+    d = make(size, torch.float32, device, seed=8, lengths=far)
+    check(call(d, size, 'NTC', grad=True), oracle(d, size, 'NTC'))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('sq', [1, 40])
+@pytest.mark.parametrize('layout', ['NTC', 'TNC'])
+def test_keys_past_2_31_elements(layout, sq):
+    """Keys of 4 GB, of which the mask leaves the first ten and the last
+    seventy, give what those eighty alone give."""
+    sk = (1 << 21) + 100
+    few, many = (1, 8, 8, sq, 80, 64), (1, 8, 8, sq, sk, 64)
+    d = make(few, torch.bfloat16, 'cuda:0', layout, seed=9)
+    shape = list(d['kv'].shape)
+    time = 1 if layout == 'NTC' else 0
+    shape[time] = sk
+    e = dict(d, kv=torch.full(shape, math.nan, dtype=torch.bfloat16,
+                              device='cuda:0'),
+             mask=torch.zeros(1, sk, dtype=torch.bool, device='cuda:0'))
+    for at, to, n in ((0, 0, 10), (10, sk - 70, 70)):
+        e['kv'].narrow(time, to, n).copy_(d['kv'].narrow(time, at, n))
+        e['mask'][:, to:to + n] = True
+    got = call(e, many, layout, grad=True)
+    rest = got[2].narrow(time, 10, sk - 80)
+    assert not rest.any()
+    got[2] = torch.cat([got[2].narrow(time, 0, 10),
+                        got[2].narrow(time, sk - 70, 70)], time)
+    check(got, oracle(d, few, layout))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('size', [(2, 4, 2, 1, 3000, 64), (2, 4, 4, 40, 90, 64)])
+def test_captured_backward(size):
+    """Forward and backward in one graph, replayed with eager work between."""
+    d = make(size, torch.bfloat16, 'cuda:0', seed=10,
+             lengths=[size[4], size[4] // 2])
+    d['length'] = d['length'].to(torch.int32)
+    call(d, size, 'NTC', grad=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        caught = call(d, size, 'NTC', grad=True)
+    for k in range(3):
+        e = make(size, torch.bfloat16, 'cuda:0', seed=20 + k)
+        for name in ('q', 'kv', 'dout'):
+            with torch.no_grad():
+                d[name].copy_(e[name])
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(caught, call(d, size, 'NTC', grad=True)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_more_refusals_on_the_gpu():
+    def zeros(*shape):
+        return nd(torch.zeros(*shape, dtype=torch.float16, device='cuda:0'))
+    f = mx.nd.contrib.encdec_attention
+    many = 1 << 24  # sequences: 2^32 threads
+    with pytest.raises(RuntimeError):
+        f(zeros(many, 1, 1), zeros(many, 1, 2))
+    heads = (1 << 20) + 1
+    with pytest.raises(RuntimeError):
+        f(zeros(1, 1, heads), zeros(1, 1, 2), heads=heads, kv_heads=1)
+    q = torch.randn(1, 2, 8, device='cuda:0', requires_grad=True)
+    kv = nd(torch.randn(1, 3, 16, device='cuda:0'))
+    with autograd.record():
+        o = f(nd(q), kv)
+    dq, = autograd.grad([o], [nd(q)], create_graph=True, retain_graph=True)
+    with pytest.raises(RuntimeError):  # no second derivatives
+        dq.to_torch().square().sum().backward()
