@@ -332,3 +332,61 @@ def test_int8_of_a_gamma_that_is_not_finite(native, device):
         q, scale = mx.nd.RMSNorm(arr(x, device), arr(g, device),
                                  out_type='int8')
         assert np.isnan(scale.asnumpy()).all() and not q.asnumpy().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['float16', 'bfloat16', 'float32'])
+def test_both_frontends_run_one_kernel(native, dtype):
+    """The native runtime gives the torch frontend's results to the bit, with
+    workspaces (split keys, rows in parts) among them."""
+    rs = np.random.RandomState(12)
+    tt = getattr(torch, dtype)
+
+    def pair(*shape, grad=False):
+        a = rs.randn(*shape).astype('float32')
+        n = mx.nd.array(a, ctx=mx.gpu(0), dtype='float32').astype(dtype)
+        t = torch.tensor(a, device='cuda:0').to(tt).requires_grad_(grad)
+        return n, mx.nd.from_torch(t)
+
+    def same(n, t):
+        n = n.astype('float32').asnumpy()
+        assert np.array_equal(n, t.to_torch().detach().float().cpu().numpy())
+
+    # (dout: what the loss passes down, the same in both)
+    q, k, dout = pair(2, 3, 256, grad=True), pair(2, 5000, 256, grad=True), \
+        pair(2, 3, 256)
+    x, res = pair(70, 256, grad=True), pair(70, 256, grad=True)
+    gamma = rs.rand(256).astype('float32')
+    gn = mx.nd.array(gamma, ctx=mx.gpu(0), dtype='float32')
+    gt = mx.nd.from_torch(torch.tensor(gamma, device='cuda:0',
+                                       requires_grad=True))
+    z, u = pair(3, 60000), rs.rand(3).astype('float32')
+    kw = dict(heads=8, kv_heads=4)
+    for v in (q[0], k[0], x[0], res[0], gn):
+        v.attach_grad()
+    with autograd.record():
+        on = mx.nd.contrib.encdec_attention(q[0], k[0], **kw)
+        yn, hn = mx.nd.RMSNorm(x[0], gn, residual=res[0])
+    autograd.backward([on, yn, hn], [dout[0], x[0], res[0]])
+    tn = mx.nd.contrib.sample_tokens(z[0], mx.nd.array(u, ctx=mx.gpu(0)),
+                                     top_p=0.8)
+    set_native(False)
+    with autograd.record():
+        ot = mx.nd.contrib.encdec_attention(q[1], k[1], **kw)
+        yt, ht = mx.nd.RMSNorm(x[1], gt, residual=res[1])
+    gq, gk = autograd.grad([ot], [q[1], k[1]], [dout[1]])
+    gx, gg = autograd.grad([yt, ht], [x[1], gt],
+                           [mx.nd.from_torch(v.to_torch().detach())
+                            for v in (x[1], res[1])])
+    t = mx.nd.contrib.sample_tokens(
+        z[1], mx.nd.from_torch(torch.tensor(u, device='cuda:0')), top_p=0.8)
+    same(on, ot)
+    same(yn, yt)
+    same(hn, ht)
+    same(q[0].grad, gq)
+    same(k[0].grad, gk)
+    same(x[0].grad, gx)
+    same(res[0].grad, gx)
+    same(gn.grad, gg)
+    same(tn, t)
+    set_native(True)
