@@ -138,27 +138,39 @@ DEV_INLINE Whole whole(double d) {
 
 DEV_INLINE int bucket(double d) { return min(whole(d).n, NB - 1); }
 
-// 2^s 2^(-d / 64), rounded to a whole number.  d = 64 q + j + f with |f| <=
-// 1/2: 2^-q is an exponent, 2^(-j / 64) comes from the table and 2^(-f / 64)
-// from its Taylor series to the 4th power (off by 4e-14 / 256 at most: the
-// powers of ln(2) / 128).  Adding 2^52 rounds it.
-DEV_INLINE u64 weight(double d, int sbits, const double* table) {
-  const Whole w = whole(d);
-  const double f = (w.f - d) * 0.010830424696249145;  // ln(2) / 64
-  double e = 1.0 / 120.0;
-  e = fma(e, f, 1.0 / 24.0);
-  e = fma(e, f, 1.0 / 6.0);
-  e = fma(e, f, 0.5);
+// 2^s 2^(-d / 64), rounded to a whole number.  d = n - f with |f| <= 1/2:
+// 2^s 2^(-n / 64) comes from the table (0 for the last bucket, whose weights
+// are less than half of one) and 2^(f / 64) from its Taylor series to the 5th
+// power (off by 4e-17 at most: (ln(2) / 128)^6 / 720).  Adding 2^52 rounds it.
+struct Weight {
+  int b;  // the bucket
+  u64 w;
+};
+DEV_INLINE Weight weight(double d, const double* table) {
+  constexpr double c = 0.010830424696249145;  // ln(2) / 64
+  const Whole n = whole(d);
+  const double f = n.f - d;
+  double e = c * c * c * c * c / 120;
+  e = fma(e, f, c * c * c * c / 24);
+  e = fma(e, f, c * c * c / 6);
+  e = fma(e, f, c * c / 2);
+  e = fma(e, f, c);
   e = fma(e, f, 1.0);
-  e = fma(e, f, 1.0);
-  e *= table[w.n & (STEP - 1)];
-  const double p =
-      __hiloint2double((1023 + sbits - (w.n / STEP)) << 20, 0);
-  return (u64)__double_as_longlong(fma(e, p, 0x1p52)) - 0x4330000000000000ull;
+  const int b = min(n.n, NB - 1);
+  return {b, (u64)__double_as_longlong(fma(e, table[b], 0x1p52)) -
+                 0x4330000000000000ull};
 }
 
-DEV_INLINE void fill_table(double* table) {
-  if (threadIdx.x < STEP) table[threadIdx.x] = exp2(threadIdx.x / -64.0);
+// the table, by all threads of a block; `octave` has room for STEP values
+template <int THREADS>
+DEV_INLINE void fill_table(double* table, double* octave, int sbits) {
+  if (threadIdx.x < STEP) octave[threadIdx.x] = exp2(threadIdx.x / -64.0);
+  __syncthreads();
+  for (int i = threadIdx.x; i < NB; i += THREADS)
+    table[i] = i == NB - 1 ? 0.0
+                           : octave[i % STEP] *
+                                 __hiloint2double(
+                                     (1023 + sbits - i / STEP) << 20, 0);
 }
 
 // the order as ascending numbers: larger logits first, then lower indices
@@ -227,10 +239,9 @@ DEV_INLINE void count_row(const Sample& a, const T* x, long i0, long i1,
   // operations overlap)
   auto each = [&](auto numbers) {
     scan<T, THREADS>(x, i0, i1, [&](long, float v) {
-      const double d = depth(v, r);
-      const int b = bucket(d);
-      if (decltype(numbers)::value) atomicAdd(&count[b], 1u);
-      atomicAdd(&mass[b], weight(d, a.sbits, table));
+      const Weight w = weight(depth(v, r), table);
+      if (decltype(numbers)::value) atomicAdd(&count[w.b], 1u);
+      atomicAdd(&mass[w.b], w.w);
     });
   };
   if (number) each(std::true_type{});
@@ -247,8 +258,10 @@ template <typename T>
 __global__ __launch_bounds__(512) void sample_count_kernel(Sample a) {
   __shared__ u64 mass[NB];
   __shared__ unsigned count[NB];
-  __shared__ double table[STEP];
-  fill_table(table);
+  __shared__ double table[NB];
+  // (a place that is read as numbers only after the next barrier)
+  fill_table<512>(table, (double*)count, a.sbits);
+  __syncthreads();
   const int n = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   for (int b = threadIdx.x; b < NB; b += 512) {
     mass[b] = 0;
@@ -276,7 +289,7 @@ struct Lds {
   // a bucket too full for the list
   u64 fine_mass[LIST];
   unsigned fine_count[LIST];
-  double table[STEP];
+  double table[NB];
   u64 wave[NT / 64];
   float bound[8];
   u64 at, through;
@@ -487,7 +500,7 @@ DEV_INLINE void gather(const Sample& a, const T* x, const Row& r, const Ask& q,
     each(least, most, [&](float v, u64 e) {
       const int k = (int)((e - least) >> shift);
       atomicAdd(&s.fine_count[k], 1u);
-      const u64 w = weight(depth(v, r), a.sbits, s.table);
+      const u64 w = weight(depth(v, r), s.table).w;
       if (w) atomicAdd(&s.fine_mass[k], w);
     });
     __syncthreads();
@@ -530,8 +543,9 @@ DEV_INLINE bool ask(const Sample& a, const T* x, const Row& r, const Ask& q,
   for (int j = 0; j < 2; ++j)
     if (i0 + j < held->n) {
       const double d = depth(entry_logit(s.list[i0 + j]), r);
-      if (bucket(d) == b) {
-        w[j] = weight(d, a.sbits, s.table);
+      const Weight e = weight(d, s.table);
+      if (e.b == b) {
+        w[j] = e.w;
         c[j] = 1;
       }
     }
@@ -568,7 +582,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(Sample a) {
   const int n = blockIdx.x, t = threadIdx.x;
   const T* x = (const T*)a.x + n * a.V;
   float top = -kInf;
-  fill_table(s.table);
+  fill_table<NT>(s.table, (double*)s.list, a.sbits);
   if constexpr (COUNTED) {
     top = parts_top(a, n);
     for (int b = t; b < NB; b += NT) {
@@ -690,7 +704,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(Sample a) {
         }
         if (v >= vb[6] && v <= vb[7]) {
           const double d = depth(v, r);
-          if (d <= most) part += weight(d, a.sbits, s.table);
+          if (d <= most) part += weight(d, s.table).w;
         }
       });
   __syncthreads();
