@@ -120,10 +120,10 @@ DEV_INLINE void scan_some(const T* x, long n, S some, F f) {
 }
 
 // How far a logit lies below the maximum, in buckets: -64 log2 of its weight,
-// at most 8000 (which weighs nothing), also for -inf and NaN.  Not increasing
-// in v, so that buckets follow the order.
+// at most the last one's number (which weighs nothing), also for -inf and NaN.
+// Not increasing in v, so that buckets follow the order.
 DEV_INLINE double depth(float v, const Row& r) {
-  return fmax(fmin((r.top - (double)v) * r.scale, 8000.0), 0.0);
+  return fmax(fmin((r.top - (double)v) * r.scale, (double)(NB - 1)), 0.0);
 }
 
 // Adding 1.5 * 2^52 rounds a double to a whole number in its lowest bits
@@ -136,7 +136,7 @@ DEV_INLINE Whole whole(double d) {
   return {(int)__double2loint(t), t - 0x1.8p52};
 }
 
-DEV_INLINE int bucket(double d) { return min(whole(d).n, NB - 1); }
+DEV_INLINE int bucket(double d) { return whole(d).n; }
 
 // 2^s 2^(-d / 64), rounded to a whole number.  d = n - f with |f| <= 1/2:
 // 2^s 2^(-n / 64) comes from the table (0 for the last bucket, whose weights
@@ -156,9 +156,8 @@ DEV_INLINE Weight weight(double d, const double* table) {
   e = fma(e, f, c * c / 2);
   e = fma(e, f, c);
   e = fma(e, f, 1.0);
-  const int b = min(n.n, NB - 1);
-  return {b, (u64)__double_as_longlong(fma(e, table[b], 0x1p52)) -
-                 0x4330000000000000ull};
+  return {n.n, (u64)__double_as_longlong(fma(e, table[n.n], 0x1p52)) -
+                   0x4330000000000000ull};
 }
 
 // the table, by all threads of a block; `octave` has room for STEP values
@@ -292,20 +291,41 @@ struct Lds {
   double table[NB];
   u64 wave[NT / 64];
   float bound[8];
-  u64 at, through;
-  int found;
   unsigned n;
+  // for each of the three questions
+  struct Answer {
+    u64 before;  // of the list, where the question's bucket begins: weight
+    int first;   // and number
+    int found;
+    u64 at, through;
+  } answer[3];
 };
+
+// v and what the lanes that CTRL (a DPP control) names hold, in the rows of
+// 16 lanes that ROWS names
+template <int CTRL, int ROWS>
+DEV_INLINE u64 add_lanes(u64 v) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(
+      0, (int)(unsigned)v, CTRL, ROWS, 0xf, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(
+      0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((u64)hi << 32 | lo);
+}
+
+// sum of the lanes up to this one
+DEV_INLINE u64 sum_lanes(u64 v) {
+  v = add_lanes<0x111, 0xf>(v);  // 1, 2, 4 and 8 lanes below, in the row
+  v = add_lanes<0x112, 0xf>(v);
+  v = add_lanes<0x114, 0xf>(v);
+  v = add_lanes<0x118, 0xf>(v);
+  v = add_lanes<0x142, 0xa>(v);  // the row below's last, for rows 1 and 3
+  return add_lanes<0x143, 0xc>(v);  // lane 31, for rows 2 and 3
+}
 
 // running sum of the threads before this one; *total: of all
 DEV_INLINE u64 sum_before(u64 v, u64* wave, u64* total) {
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  u64 in = v;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const u64 p = (u64)__shfl_up(in, off, 64);
-    if (l >= off) in += p;
-  }
+  const u64 in = sum_lanes(v);
   if (l == 63) wave[w] = in;
   __syncthreads();
   u64 b = 0, all = 0;
@@ -340,6 +360,7 @@ struct Ask {
     kOver,    // ... whose running weight is over want
   } kind;
   double want;
+  int index;  // which of the answers is its own
 };
 
 DEV_INLINE bool reached(const Ask& q, u64 through) {
@@ -431,12 +452,33 @@ DEV_INLINE void sort_list(Lds& s, int n) {
   __syncthreads();
 }
 
-// what the list holds, in order: n entries, those of the buckets lo[i] to
-// hi[i] (none where lo > hi) among them all
+// What the list holds, in order: n entries, those of the buckets lo[i] to
+// hi[i] (none where lo > hi) among them all; and this thread's two of them
 struct Held {
   int lo[3], hi[3];
   int n;
+  int b[2];      // their buckets (NB: no entry),
+  int before;    // that of the one before them (-1: none)
+  u64 w[2], sum; // weights, and the list's running sum before them
 };
+
+DEV_INLINE void weigh_list(Lds& s, const Row& r, Held* held) {
+  const int i0 = threadIdx.x * 2;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    held->b[j] = NB;
+    held->w[j] = 0;
+    if (i0 + j < held->n) {
+      const Weight e = weight(depth(entry_logit(s.list[i0 + j]), r), s.table);
+      held->b[j] = e.b;
+      held->w[j] = e.w;
+    }
+  }
+  held->before = i0 > 0 && i0 < held->n
+                     ? bucket(depth(entry_logit(s.list[i0 - 1]), r)) : -1;
+  u64 all;
+  held->sum = sum_before(held->w[0] + held->w[1], s.wave, &all);
+}
 
 // Brings the one bucket b to the list; where that cannot hold it (many equal
 // logits), the part of it in which the question is reached, and *weight0 and
@@ -515,9 +557,10 @@ DEV_INLINE void gather(const Sample& a, const T* x, const Row& r, const Ask& q,
     lo = least + ((u64)k << shift);
     hi = min(most, lo + ((1ull << shift) - 1));
   }
-  const int n = (int)s.n;
-  sort_list(s, n);
-  *held = Held{{whole_bucket ? b : 0, 0, 0}, {whole_bucket ? b : -1, -1, -1}, n};
+  *held = Held{{whole_bucket ? b : 0, 0, 0}, {whole_bucket ? b : -1, -1, -1},
+               (int)s.n};
+  sort_list(s, held->n);
+  weigh_list(s, r, held);
 }
 
 // The question's entry, and the weight through it.  False where it lies in the
@@ -535,45 +578,35 @@ DEV_INLINE bool ask(const Sample& a, const T* x, const Row& r, const Ask& q,
 #pragma unroll
   for (int i = 0; i < 3; ++i) have |= held->lo[i] <= b && b <= held->hi[i];
   if (!have) gather(a, x, r, q, b, s, held, &weight0, &number0);
-  // two entries to a thread; the ones of other buckets do not count
+  // the bucket's entries follow each other: the first tells where they begin
+  Lds::Answer& mine = s.answer[q.index];
   const int i0 = threadIdx.x * 2;
-  u64 w[2] = {0, 0};
-  unsigned c[2] = {0, 0};
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (i0 + j < held->n) {
-      const double d = depth(entry_logit(s.list[i0 + j]), r);
-      const Weight e = weight(d, s.table);
-      if (e.b == b) {
-        w[j] = e.w;
-        c[j] = 1;
-      }
-    }
-  if (threadIdx.x == 0) s.found = LIST;
-  u64 all, m = weight0 + sum_before(w[0] + w[1], s.wave, &all);
-  u64 k = number ? number0 + sum_before(c[0] + c[1], s.wave, &all) : 0;
-  int hit = LIST;
+  const bool first[2] = {held->b[0] == b && held->before != b,
+                         held->b[1] == b && held->b[0] != b};
+  if (first[0] || first[1]) {
+    mine.before = held->sum + (first[1] ? held->w[0] : 0);
+    mine.first = i0 + first[1];
+  }
+  __syncthreads();
+  // running number and weight before each entry: one entry is the first with
+  // which the question is reached
+  u64 k = number0 + (i0 - mine.first), m = weight0 + held->sum - mine.before;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    m += w[j];
-    k += c[j];
-    if (hit == LIST && c[j] && reached(q, number ? k : m)) {
-      hit = i0 + j;
-      w[0] = m;  // (taken already)
+    const u64 k1 = k + 1, m1 = m + held->w[j];
+    if (held->b[j] == b && reached(q, number ? k1 : m1) &&
+        (first[j] || !reached(q, number ? k : m))) {
+      mine.at = s.list[i0 + j];
+      mine.through = m1;
+      mine.found = 1;
     }
-  }
-  if (hit < LIST) atomicMin(&s.found, hit);
-  __syncthreads();
-  const int first = s.found;
-  if (first < LIST && first == hit) {
-    s.at = s.list[first];
-    s.through = w[0];
+    k = k1;
+    m = m1;
   }
   __syncthreads();
-  *at = s.at;
-  *through = s.through;
-  __syncthreads();
-  return first < LIST;
+  *at = mine.at;
+  *through = mine.through;
+  return mine.found;
 }
 
 template <typename T, bool COUNTED>
@@ -582,6 +615,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(Sample a) {
   const int n = blockIdx.x, t = threadIdx.x;
   const T* x = (const T*)a.x + n * a.V;
   float top = -kInf;
+  if (t < 3) s.answer[t].found = s.answer[t].first = 0;
   fill_table<NT>(s.table, (double*)s.list, a.sbits);
   if constexpr (COUNTED) {
     top = parts_top(a, n);
@@ -625,7 +659,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(Sample a) {
   const float u = fmaxf(fminf(a.u[n], 1.f - 0x1p-24f), 0.f);
   u64 keep = s.mass[NB - 1], keep0 = keep, keep1 = keep;
   Held held = {{0, 0, 0}, {-1, -1, -1}, 0};
-  const Ask ask_k = {Ask::kNumber, (double)k};
+  const Ask ask_k = {Ask::kNumber, (double)k, 0};
   if (k) {
     const int b = find_bucket(ask_k, s);
     if (b < NB - 1) {
@@ -636,8 +670,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(Sample a) {
   }
   const double want_p = fmax(p, 0.0);
   if (p < 1.0) {
-    const int b0 = find_bucket(Ask{Ask::kWeight, want_p * (double)keep0}, s),
-              b1 = find_bucket(Ask{Ask::kWeight, want_p * (double)keep1}, s);
+    const int b0 = find_bucket(Ask{Ask::kWeight, want_p * (double)keep0, 1}, s),
+              b1 = find_bucket(Ask{Ask::kWeight, want_p * (double)keep1, 1}, s);
     held.lo[1] = b0;
     held.hi[1] = min(b1, NB - 2);
     keep0 = min(keep0, before(s.mass, b0));
@@ -651,9 +685,9 @@ __global__ __launch_bounds__(NT) void sample_kernel(Sample a) {
     keep0 = min(keep0, before(s.mass, bm));
     keep1 = min(keep1, s.mass[bm]);
   }
-  held.lo[2] = find_bucket(Ask{Ask::kOver, (double)u * (double)keep0}, s);
+  held.lo[2] = find_bucket(Ask{Ask::kOver, (double)u * (double)keep0, 2}, s);
   held.hi[2] = min(
-      find_bucket(Ask{Ask::kOver, (double)u * (double)keep1}, s), NB - 2);
+      find_bucket(Ask{Ask::kOver, (double)u * (double)keep1, 2}, s), NB - 2);
 
   // one scan for them all: a wave finds each end of each range
   if (t < 8 * 64) {
@@ -709,22 +743,24 @@ __global__ __launch_bounds__(NT) void sample_kernel(Sample a) {
       });
   __syncthreads();
   held.n = (int)s.n;
-  if (held.n <= LIST)
+  if (held.n <= LIST) {
     sort_list(s, held.n);
-  else  // too many: each question brings its own
+    weigh_list(s, r, &held);
+  } else {  // too many: each question brings its own
     held = Held{{0, 0, 0}, {-1, -1, -1}, 0};
+  }
 
   u64 at = 0, sum;
   if (k && ask(a, x, r, ask_k, s, &held, &at, &sum)) keep = sum;
-  if (p < 1.0 && ask(a, x, r, Ask{Ask::kWeight, want_p * (double)keep}, s,
-                     &held, &at, &sum))
+  if (p < 1.0 && ask(a, x, r, Ask{Ask::kWeight, want_p * (double)keep, 1},
+                     s, &held, &at, &sum))
     keep = min(keep, sum);
   if (limit) {
     sum_before(part, s.wave, &sum);
     keep = min(keep, before(s.mass, bm) + sum);
   }
-  const bool got = ask(a, x, r, Ask{Ask::kOver, (double)u * (double)keep}, s,
-                       &held, &at, &sum);
+  const bool got = ask(a, x, r, Ask{Ask::kOver, (double)u * (double)keep, 2},
+                       s, &held, &at, &sum);
   if (t == 0) {
     a.token[n] = got ? (int)(unsigned)at : -1;
     if (a.logp) {
