@@ -62,9 +62,9 @@ struct Row {
 };
 
 // f(index, 16 bytes of logits) and g(index, logit) over [i0, i1) by the
-// block's threads, the first where the memory is aligned.  (Four loads on
-// their way at once gained nothing at 256 rows of 131072, whose 16 waves hide
-// them, and lost 4 us at 32 rows of 30522 to the longer code.)
+// block's threads, the first where the memory is aligned.  The next two loads
+// are on their way while f looks at one (256 rows of 131072: 65 us to 64; at
+// 32 of 30522, 24 us either way).
 template <typename T, int THREADS, typename F, typename G>
 DEV_INLINE void scan_vectors(const T* x, long i0, long i1, F f, G g) {
   constexpr int N = 16 / sizeof(T);
@@ -73,8 +73,17 @@ DEV_INLINE void scan_vectors(const T* x, long i0, long i1, F f, G g) {
       min(i1, i0 + (long)((-(uintptr_t)(x + i0) & 15) / sizeof(T)));
   const long nv = (i1 - a) / N;
   for (long i = i0 + threadIdx.x; i < a; i += THREADS) g(i, (float)x[i]);
-  for (long k = threadIdx.x; k < nv; k += THREADS)
-    f(a + k * N, *(const VecT*)(x + a + k * N));
+  const VecT* p = (const VecT*)(x + a);
+  long k = threadIdx.x;
+  if (k < nv) {
+    VecT v0 = p[k], v1 = p[min(k + THREADS, nv - 1)];
+    for (; k < nv; k += THREADS) {
+      const VecT v = v0;
+      v0 = v1;
+      v1 = p[min(k + 2 * THREADS, nv - 1)];
+      f(a + k * N, v);
+    }
+  }
   for (long i = a + nv * N + threadIdx.x; i < i1; i += THREADS)
     g(i, (float)x[i]);
 }
