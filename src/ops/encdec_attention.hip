@@ -1015,31 +1015,37 @@ int splits(long blocks, long want, long tiles, long least) {
   return (int)std::max<long>(1, std::min<long>(n, 64));
 }
 
+constexpr int NW = 4;  // waves of rows (keys for dK and dV) in a block
+
 struct Plan {
-  int DP, NW, fwd, dq, dkv, kw;  // waves of rows, splits, waves of keys
+  int DP;
+  bool token;         // the forward's kernel for at most 32 rows
+  int fwd, dq, dkv;   // splits
 };
 
-// NW = 0: the kernel for single tokens.
-// Two blocks a CU (512) are wanted: twice that, to even out sequences of
-// different lengths, gained nothing (one token of 8x32 heads over 8192 to
-// 16384 keys: 87 us to 85).
+// Up to 32 rows that share a key head, the kernel for single tokens (14 us
+// against 17 for 32x16 heads over 512 keys of 64, 85 against 107 for 8x8 heads
+// of four rows over 16384 of 128; at 32 rows over 128 keys both take 7).
+// Blocks of two waves for 64 rows or keys gained nothing over four.
+//
+// One block a CU (256) is wanted: 512 rows of 8 heads over 4096 keys of 64
+// take 22 us forward and 45 back with 256, 24 and 59 with 512, 70 and 96 with
+// no split.  Single tokens, whose time is their longest sequence's, want twice
+// that (8 sequences of up to 16384 keys: 75 us, and 79 with 256).
 // A split costs a launch and its partial results, so it has four tiles (about
-// 4 us) or more; one tile in fp32, whose products take 16 times as long.
+// 4 us) or more, eight of single tokens; one tile in fp32, whose products take
+// 16 times as long.
 Plan make_plan(long B, long H, long Hk, long Sq, long Sk, long D, int dtype) {
   Plan p;
-  const long M = H / Hk * Sq, bh = B * Hk;
+  const long M = H / Hk * Sq, bh = B * Hk, tile = NW * 32;
   const long least = dtype == kFloat32 ? 1 : 4;
-  p.DP = pad_dim((int)D);
-  p.NW = M <= 32 ? 0 : M <= 64 ? 2 : 4;
-  const int rows = std::max(p.NW, 1) * 32;
+  const long rows = bh * ((M + tile - 1) / tile);
   const long tiles = (Sk + 63) / 64;
-  p.fwd = splits(bh * ((M + rows - 1) / rows), 512, tiles,
-                 p.NW ? least : 8);
-  const int qrows = p.NW == 4 ? 128 : 64;
-  p.dq = splits(bh * ((M + qrows - 1) / qrows), 512, tiles, least);
-  p.kw = Sk <= 64 ? 2 : 4;
-  p.dkv = splits(bh * ((Sk + p.kw * 32 - 1) / (p.kw * 32)), 512,
-                 (M + 63) / 64, least);
+  p.DP = pad_dim((int)D);
+  p.token = M <= 32;
+  p.fwd = p.token ? splits(bh, 512, tiles, 8) : splits(rows, 256, tiles, least);
+  p.dq = splits(rows, 256, tiles, least);
+  p.dkv = splits(bh * ((Sk + tile - 1) / tile), 256, (M + 63) / 64, least);
   return p;
 }
 
@@ -1145,18 +1151,16 @@ void fwd(const LaunchCtx& lc, Att a, const Plan& p) {
   const long bh = (long)a.B * a.Hk, M = (long)a.G * a.Sq;
   by_dim(p.DP, [&](auto dp) {
     constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>();
-    const unsigned n = grid(bh * a.nsplit *
-                            (p.NW ? (M + p.NW * 32 - 1) / (p.NW * 32) : 1));
-    if (p.NW == 0)
+    const unsigned n = grid(
+        bh * a.nsplit * (p.token ? 1 : (M + NW * 32 - 1) / (NW * 32)));
+    if (p.token)
       // a wave's own tile of 16 KB at most.  (Tiles of 32 keys in blocks of
       // eight waves, four a SIMD: 21 us for 32x16 heads over 512 keys of 64,
       // where this takes 17.)
       att_token_kernel<T, DP, sizeof(T) == 2 && DP <= 64 ? 64 : 32>
           <<<n, 256, 0, lc.stream>>>(a);
-    else if (p.NW == 2)
-      att_fwd_kernel<T, DP, 2, BN><<<n, 128, 0, lc.stream>>>(a);
     else
-      att_fwd_kernel<T, DP, 4, BN><<<n, 256, 0, lc.stream>>>(a);
+      att_fwd_kernel<T, DP, NW, BN><<<n, NW * 64, 0, lc.stream>>>(a);
   });
   if (a.nsplit > 1)
     att_join_kernel<T><<<grid((bh * M + 3) / 4), 256, 0, lc.stream>>>(a, p.DP);
@@ -1170,13 +1174,8 @@ void bwd(const LaunchCtx& lc, Att a, const Plan& p) {
     a.nsplit = p.dq;
     by_dim(p.DP, [&](auto dp) {
       constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>();
-      if (p.NW == 4)
-        att_dq_kernel<T, DP, 4, BN>
-            <<<grid(bh * a.nsplit * ((M + 127) / 128)), 256, 0, lc.stream>>>(
-                a);
-      else
-        att_dq_kernel<T, DP, 2, BN>
-            <<<grid(bh * a.nsplit * ((M + 63) / 64)), 128, 0, lc.stream>>>(a);
+      const unsigned n = grid(bh * a.nsplit * ((M + NW * 32 - 1) / (NW * 32)));
+      att_dq_kernel<T, DP, NW, BN><<<n, NW * 64, 0, lc.stream>>>(a);
     });
     if (a.nsplit > 1)
       att_dq_join_kernel<T>
@@ -1186,12 +1185,9 @@ void bwd(const LaunchCtx& lc, Att a, const Plan& p) {
     a.nsplit = p.dkv;
     by_dim(p.DP, [&](auto dp) {
       constexpr int DP = decltype(dp)::value, BN = tile_rows<T, DP>();
-      const int keys = p.kw * 32;
-      const unsigned n = grid(bh * a.nsplit * ((a.Sk + keys - 1) / keys));
-      if (p.kw == 4)
-        att_dkv_kernel<T, DP, 4, BN><<<n, 256, 0, lc.stream>>>(a);
-      else
-        att_dkv_kernel<T, DP, 2, BN><<<n, 128, 0, lc.stream>>>(a);
+      const unsigned n =
+          grid(bh * a.nsplit * ((a.Sk + NW * 32 - 1) / (NW * 32)));
+      att_dkv_kernel<T, DP, NW, BN><<<n, NW * 64, 0, lc.stream>>>(a);
     });
     if (a.nsplit > 1)
       att_dkv_join_kernel<T>

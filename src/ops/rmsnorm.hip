@@ -410,9 +410,13 @@ __global__ __launch_bounds__(1024) void rms_dgamma_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// which variant: the smallest number of threads whose registers hold the row
-// (a wave a row needs no barrier, but a launch of few rows wants the whole
-// block on each, or most of the chip idles)
+// Which variant: the smallest number of threads whose registers hold the row.
+// A wave a row needs no barrier, but a launch of few rows wants a whole block
+// on each, or most of the chip idles.  In bf16, forward and backward in us,
+// a wave a row against a block:
+//   512 rows of 768  3.3, 6.8 against 3.1, 6.3     of 2048  4.5, 9.2, 3.7, 7.9
+//   1024 rows        3.4, 6.9 against 3.5, 7.4              5.0, 9.4, 4.3, 9.4
+//   4096 rows        5.3, 10.0 against 7.4, 16.0            11, 18.5, 12, 22
 // ---------------------------------------------------------------------------
 struct RowPlan {
   int tpr = 0, nv = 0;  // 0: the kernel that reads the row again
@@ -578,10 +582,14 @@ void rms_norm_fwd_raw(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
   HIP_CHECK_LAST();
 }
 
-// two blocks for each of 256 CUs, and no more than there are rows for: the
-// partials are nblk rows to write and to read again
+// Two blocks for each of 256 CUs, and no more than there are rows; four from
+// 16384 rows on, of which a block then has 16 or more (768 columns: 25 us
+// against 29 with two, 4096: 99 against 105, 2048: 53 against 52), since the
+// partials are a row a block to write and to read again (4096 rows of 768:
+// 10.7 us with four, 10.0 with two).
 int64_t rms_norm_bwd_blocks(int64_t rows) {
-  return std::max<int64_t>(1, std::min<int64_t>(rows, 512));
+  return std::max<int64_t>(1,
+                           std::min<int64_t>(rows, rows < 16384 ? 512 : 1024));
 }
 
 void rms_norm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,

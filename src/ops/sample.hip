@@ -793,9 +793,13 @@ void launch(const LaunchCtx& lc, const Sample& a) {
 }
 
 // Parts of a row: enough blocks for the chip, none with less than 4096
-// logits; 1 where a block a row is enough
+// logits; 1, and one launch, where the rows are short or many.  In us, one
+// launch against three, bf16:
+//   V = 65536:  1 row 34, 31      8 rows 34, 34     32 rows 36, 42
+//   V = 131072: 1 row 51, 39     64 rows 56, 52    128 rows 57, 61
+//   V = 262144: 1 row 88, 56     64 rows 98, 79    128 rows 104, 95
 int parts_of(int64_t N, int64_t V) {
-  if (V <= 32768 || N >= 192) return 1;
+  if (V - 1024 * N < 56 << 10) return 1;
   return (int)std::max<int64_t>(1, std::min(512 / std::max<int64_t>(N, 1),
                                             V / 4096));
 }

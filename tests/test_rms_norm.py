@@ -380,3 +380,23 @@ def test_second_derivatives_are_refused():
                         retain_graph=True)
     with pytest.raises(RuntimeError):
         dx.to_torch().square().sum().backward()
+
+
+@pytest.mark.gpu
+def test_gradient_of_many_rows():
+    """dgamma's partials of twice as many blocks; sums of 16400 products of
+    values of order one in 32 bits, in an order of the kernel's own."""
+    rows, cols = 16400, 64
+    d = make(rows, cols, torch.float32, 'cuda:0', seed=14)
+    x, gamma = (mx.nd.from_torch(d[k].requires_grad_()) for k in ('x', 'gamma'))
+    with autograd.record():
+        y = mx.nd.RMSNorm(x, gamma)
+    dx, dg = autograd.grad([y], [x, gamma], [mx.nd.from_torch(d['dy'])])
+    h, g, dy = (d[k].detach().double() for k in ('x', 'gamma', 'dy'))
+    r = 1 / torch.sqrt(h.square().mean(-1, keepdim=True) + 1e-6)
+    n, t = h * r, dy * g
+    want = r * (t - n * (t * n).mean(-1, keepdim=True))
+    within(dx.to_torch(), want, r * (t.abs() + n.abs() * (
+        t * n).abs().mean(-1, keepdim=True)) * (cols + 8) * U32)
+    within(dg.to_torch(), (dy * n).sum(0), (dy * n).abs().sum(0)
+           * (rows + 8) * U32)

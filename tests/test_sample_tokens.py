@@ -252,3 +252,45 @@ def test_past_2_31_logits():
     alone = mx.nd.contrib.sample_tokens(nd(last), nd(u[-3:].clone()), **kw)
     assert torch.equal(token.to_torch()[-3:], alone[0].to_torch())
     assert torch.equal(logp.to_torch()[-3:], alone[1].to_torch())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+def test_long_rows_in_parts(dtype, device):
+    """Few rows of many logits, which the kernels count in parts."""
+    x, u = make(4, 70001, dtype, device, seed=13)
+    x[1, ::3] = -math.inf
+    x[1, 69990:] = math.nan
+    x[2] = math.nan
+    x[3] = 0.25
+    for kw in ({}, dict(top_k=60, top_p=0.9), dict(min_p=0.05),
+               dict(temperature=0.0), dict(top_k=30000, top_p=0.7)):
+        check(x, u, **kw)
+    check(x, u, temperature=torch.tensor([0.5, 1, 2, 0], device=device),
+          top_k=torch.tensor([0, 5, 0, 9], dtype=torch.int32, device=device))
+
+
+@pytest.mark.gpu
+def test_graphs_of_long_rows():
+    """Two captured calls with workspaces, replayed in turn."""
+    xs = [torch.randn(2, 80000, device='cuda:0') * 3 for _ in range(2)]
+    u = torch.rand(2, device='cuda:0')
+    kw = dict(top_p=0.8, top_k=1000, get_prob=True)
+    graphs, outs = [], []
+    for v in xs:
+        mx.nd.contrib.sample_tokens(nd(v), nd(u), **kw)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(mx.nd.contrib.sample_tokens(nd(v), nd(u), **kw))
+        graphs.append(g)
+    for k in range(3):
+        u.uniform_()
+        for v in xs:
+            v.normal_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for v, o in zip(xs, outs):
+            e = mx.nd.contrib.sample_tokens(nd(v), nd(u), **kw)
+            for a, b in zip(o, e):
+                assert np.array_equal(a.asnumpy(), b.asnumpy())
