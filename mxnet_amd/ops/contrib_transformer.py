@@ -91,7 +91,7 @@ class _EncDecAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_nn.once_differentiable
     def backward(ctx, dout):
         q, kv, values, length, mask, out, lse = ctx.saved_tensors
         heads, kv_heads, tnc = ctx.conf

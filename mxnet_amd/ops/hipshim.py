@@ -464,8 +464,7 @@ def rms_norm_fwd(x, gamma, residual, eps, int8=False, want_stat=True):
     want_stat, where no backward follows)."""
     x = _c(x)
     dev, s = _dev_stream(x)
-    y = torch.empty(x.shape, dtype=torch.int8 if int8 else x.dtype,
-                    device=x.device)
+    y = torch.empty_like(x, dtype=torch.int8) if int8 else torch.empty_like(x)
     stat = torch.empty(x.shape[:-1] + (1,), dtype=torch.float32,
                        device=x.device) if want_stat else None
     res = _c(residual) if residual is not None else None
@@ -483,14 +482,14 @@ def rms_norm_bwd(dy, dsum, h, gamma, rstd):
     C = h.shape[-1]
     rows = h.numel() // C
     dx = torch.empty_like(h)
-    dgamma = torch.empty((C,), dtype=torch.float32, device=h.device)
-    partial = torch.empty((_raw.rms_norm_bwd_blocks(rows), C),
-                          dtype=torch.float32, device=h.device)
+    g = _f32(gamma)
+    dgamma = torch.empty_like(g)
+    partial = rstd.new_empty((_raw.rms_norm_bwd_blocks(rows), C))
     _raw.rms_norm_bwd(dev, s, _arr(dy),
                       _arr(_c(dsum)) if dsum is not None else None, _arr(h),
-                      _arr(_f32(gamma)), _arr(rstd), _arr(dx), _arr(dgamma),
+                      _arr(g), _arr(rstd), _arr(dx), _arr(dgamma),
                       _arr(partial))
-    return dx, dgamma.to(gamma.dtype)
+    return dx, dgamma if g is gamma else dgamma.to(gamma.dtype)
 
 
 # ---------------------------------------------------------------------------

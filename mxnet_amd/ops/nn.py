@@ -594,6 +594,18 @@ def layer_norm(x, gamma, beta, axis=-1, eps=1e-5):
     return y.to(x.dtype)
 
 
+def once_differentiable(backward):
+    """torch's decorator of that name, whose bookkeeping (2 us a call) is left
+    out where no graph is made of the backward pass."""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        f = checked if torch.is_grad_enabled() else backward
+        return f(ctx, *grads)
+    return run
+
+
 class _RMSNorm(torch.autograd.Function):
     """Fused (residual addition +) root-mean-square norm of the last axis;
     both outputs are differentiable."""
@@ -608,7 +620,7 @@ class _RMSNorm(torch.autograd.Function):
         return y if residual is None else (y, total)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dy, dsum=None):
         h, gamma, rstd = ctx.saved_tensors
         if dy is None:  # only the sum was used
