@@ -267,8 +267,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   float dg[NV][VEC] = {};
   // a row is on its way while the one before is reduced (16384x4096 bf16:
-  // 112 us, 127 without), where the registers hold two
-  constexpr bool AHEAD = TPR < 1024;
+  // 112 us, 127 without), where the registers hold two.  Elsewhere they do not
+  // hold dsum beside the row either: it is read where it is added
+  constexpr bool AHEAD = TPR < 1024 || NV <= 2;
   VecT a[NV], b[NV], e[NV], na[NV], nb[NV], ne[NV];
   float r = 0.f, nr = 0.f;
   const long step = (long)gridDim.x * RPB;
@@ -281,7 +282,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
       if (c < C) {
         na[i] = __builtin_nontemporal_load((const VecT*)(dy + base + c));
         nb[i] = *(const VecT*)(h + base + c);
-        if constexpr (DSUM)
+        if constexpr (DSUM && AHEAD)
           ne[i] = __builtin_nontemporal_load((const VecT*)(dsum + base + c));
       }
     }
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
     for (int i = 0; i < NV; ++i) {
       a[i] = na[i];
       b[i] = nb[i];
-      if constexpr (DSUM) e[i] = ne[i];
+      if constexpr (DSUM && AHEAD) e[i] = ne[i];
     }
     if (AHEAD && row + step < rows) fetch(row + step);
     float m = 0.f;
@@ -314,11 +315,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
       }
     }
     m = row_sum_f32<TPR>(m, red) / C;
+    // (without this the compiler keeps the row's products for the loop below,
+    // in scratch memory where the registers do not hold them: 32768 columns)
+    if constexpr (!AHEAD && VEC > 1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        asm volatile("" : "+v"(*(int4_t*)&a[i]), "+v"(*(int4_t*)&b[i]));
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
       if (c < C) {
         const VecG g = *(const VecG*)(gamma + c);
+        if constexpr (DSUM && !AHEAD)
+          e[i] = __builtin_nontemporal_load((const VecT*)(dsum + base + c));
         VecT o;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -449,6 +459,7 @@ RowPlan plan_rows(long rows, int C, size_t size, bool aligned) {
     fits(256, 1);
     fits(256, 2);
     fits(256, 4);
+    fits(1024, 2);
     fits(1024, 4);
   } else {
     fits(64, 4);
@@ -474,6 +485,7 @@ RowPlan plan_rows(long rows, int C, size_t size, bool aligned) {
   RMS_CASE(FULL, 256, 1) \
   RMS_CASE(FULL, 256, 2) \
   RMS_CASE(FULL, 256, 4) \
+  RMS_CASE(FULL, 1024, 2) \
   RMS_CASE(FULL, 1024, 4) \
   RMS_CASE(1, 64, 4) \
   RMS_CASE(1, 256, 4) \

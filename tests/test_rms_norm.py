@@ -400,3 +400,41 @@ def test_gradient_of_many_rows():
         t * n).abs().mean(-1, keepdim=True)) * (cols + 8) * U32)
     within(dg.to_torch(), (dy * n).sum(0), (dy * n).abs().sum(0)
            * (rows + 8) * U32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('with_res', [False, True])
+@pytest.mark.parametrize('rows,cols', [(3, 12288), (600, 9000), (2, 20000),
+                                       (5, 32768), (3, 9001)])
+def test_wide_rows(rows, cols, with_res, dtype):
+    """A block of 1024 threads a row, with one row ahead or without."""
+    test_forward(rows, cols, with_res, dtype, 'cuda:0')
+    test_gradient(rows, cols, with_res, dtype, 'cuda:0')
+
+
+@pytest.mark.gpu
+def test_captured_backward():
+    d = make(64, 768, torch.float16, 'cuda:0', seed=15)
+
+    def call():
+        x, res, gamma = (mx.nd.from_torch(d[k].detach().requires_grad_())
+                         for k in ('x', 'res', 'gamma'))
+        with autograd.record():
+            y, h = mx.nd.RMSNorm(x, gamma, residual=res)
+        grads = autograd.grad([y, h], [x, res, gamma],
+                              [mx.nd.from_torch(d[k]) for k in ('dy', 'dsum')])
+        return [t.to_torch().detach() for t in [y, h] + grads]
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        caught = call()
+    for k in range(3):
+        e = make(64, 768, torch.float16, 'cuda:0', seed=30 + k)
+        for name in ('x', 'res', 'dy', 'dsum'):
+            d[name].copy_(e[name])
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(caught, call()):
+            assert torch.equal(a, b)
