@@ -26,7 +26,7 @@
 //
 // Measured at 4x16 heads, 1024 over 2048 keys, all of them kept, bf16:
 //   head size 64:   forward 61 us (560 TFLOP/s), backward 186 us (460)
-//   head size 128:  forward 101 us (680), backward 429 us (400)
+//   head size 128:  forward 101 us (680), backward 412 us (417)
 // and in fp32 at 2x16 heads, 1024 over 1024 keys of 64: 83 us (104), 270 us
 // (79).  A large library product reaches 1198 in bf16, 154 in fp32.  Long
 // 16-bit rows are bound by what surrounds the products: a wave spends 980
@@ -824,6 +824,14 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
     constexpr int buf = decltype(number)::value;
     if (i + 1 < t1) kt.load(i + 1);
     float16_t s[KB], dp[KB];
+    if constexpr (DP > 64) {
+      // (16 moves a tile: kept, these registers put others into scratch memory;
+      // backward of 4x16 heads, 1024 over 2048 keys of 128: 412 us, 429)
+      float d = -delta;
+      asm volatile("" : "+v"(d));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) less[j] = d;
+    }
     scores<T, DP, KB>(lk[buf], qf, s, l, float16_t{});
     scores<T, DP, KB>(lv[buf], gf, dp, l, less);
     if (kt.partial(i)) drop_keys<KB>(lkeep[buf], s, h);
