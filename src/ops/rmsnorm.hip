@@ -113,21 +113,59 @@ DEV_INLINE signed char to_int8(float v) {
   return q == q ? (signed char)q : (signed char)0;
 }
 
+// VEC elements of a row, of which `left` are there: aligned to 16 bytes and
+// all there, or (LOOSE) neither.  The hardware reads and writes vectors at any
+// element's address; a row's last ones go one by one, and zeros fill them up
+// (4096 rows of 4097 in bf16, forward and backward: 24 us and 46, where all
+// elements one by one take 50 and 92, and 4096 columns 19 and 32).
+template <typename T, int VEC>
+using Vec = T __attribute__((ext_vector_type(VEC)));
+
+template <int VEC, bool LOOSE, bool ONCE = false, typename T>
+DEV_INLINE Vec<T, VEC> load_vec(const T* p, int left) {
+  using V = Vec<T, VEC>;
+  typedef V U __attribute__((aligned(sizeof(T))));
+  if constexpr (!LOOSE)
+    return ONCE ? __builtin_nontemporal_load((const V*)p) : *(const V*)p;
+  if (left >= VEC) return *(const U*)p;
+  V v = {};
+#pragma unroll
+  for (int j = 0; j < VEC; ++j)
+    if (j < left) v[j] = p[j];
+  return v;
+}
+
+template <int VEC, bool LOOSE, typename T>
+DEV_INLINE void store_vec(T* p, int left, Vec<T, VEC> v) {
+  typedef Vec<T, VEC> U __attribute__((aligned(sizeof(T))));
+  if constexpr (!LOOSE) {
+    *(Vec<T, VEC>*)p = v;
+    return;
+  }
+  if (left >= VEC) {
+    *(U*)p = v;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j)
+    if (j < left) p[j] = v[j];
+}
+
 // ---------------------------------------------------------------------------
 // forward, the row in registers: TPR threads a row, NV vectors a thread.
 // 32x1024 in fp16 (a step of decoding) takes 3.2 us, a launch's own time;
 // 8192x1024 in bf16 to int8, 15.5 us (3.8 TB/s: 59 MB, partly from the cache).
 // ---------------------------------------------------------------------------
-template <typename T, int VEC, int TPR, int NV, bool RES, bool INT8>
+template <typename T, int VEC, int TPR, int NV, bool LOOSE, bool RES, bool INT8>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
     const T* __restrict__ x, const T* __restrict__ res,
     const float* __restrict__ gamma, T* __restrict__ y,
     signed char* __restrict__ q, float* __restrict__ scale,
     T* __restrict__ sum, float* __restrict__ rstd, long rows, int C,
     double eps) {
-  using VecT = T __attribute__((ext_vector_type(VEC)));
-  using VecG = float __attribute__((ext_vector_type(VEC)));
-  using VecQ = signed char __attribute__((ext_vector_type(VEC)));
+  using VecT = Vec<T, VEC>;
+  using VecG = Vec<float, VEC>;
+  using VecQ = Vec<signed char, VEC>;
   constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
   __shared__ double red[TPR > 64 ? TPR / 64 : 1];
   const int lane = threadIdx.x % TPR;
@@ -138,7 +176,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + lane) * VEC;
-    if (c < C) h[i] = *(const VecT*)(x + base + c);
+    if (c < C) h[i] = load_vec<VEC, LOOSE>(x + base + c, C - c);
   }
   double s = 0;
 #pragma unroll
@@ -146,10 +184,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
     const int c = (i * TPR + lane) * VEC;
     if (c < C) {
       if constexpr (RES) {
-        const VecT r = *(const VecT*)(res + base + c);
+        const VecT r = load_vec<VEC, LOOSE>(res + base + c, C - c);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) h[i][j] = (T)((float)h[i][j] + (float)r[j]);
-        *(VecT*)(sum + base + c) = h[i];
+        store_vec<VEC, LOOSE>(sum + base + c, C - c, h[i]);
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -166,11 +204,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
       if (c < C) {
-        const VecG g = *(const VecG*)(gamma + c);
+        const VecG g = load_vec<VEC, LOOSE>(gamma + c, C - c);
         VecT o;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) o[j] = (T)((float)h[i][j] * r * g[j]);
-        *(VecT*)(y + base + c) = o;
+        store_vec<VEC, LOOSE>(y + base + c, C - c, o);
       }
     }
   } else {
@@ -180,7 +218,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
       if (c < C) {
-        const VecG g = *(const VecG*)(gamma + c);
+        const VecG g = load_vec<VEC, LOOSE>(gamma + c, C - c);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           v[i][j] = (float)h[i][j] * r * g[j];
@@ -199,14 +237,14 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
         VecQ o;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) o[j] = to_int8(v[i][j] * inv);
-        *(VecQ*)(q + base + c) = o;
+        store_vec<VEC, LOOSE>(q + base + c, C - c, o);
       }
     }
   }
 }
 
-// forward of rows that no register variant holds (over 32768 16-bit columns,
-// or 16384 unaligned ones): the row is read again, from the cache
+// forward of rows that no register variant holds (over 32768 columns of 16
+// bits, 16384 of 32): the row is read again, from the cache
 template <typename T, bool RES, bool INT8>
 __global__ __launch_bounds__(1024) void rms_fwd_long_kernel(
     const T* __restrict__ x, const T* __restrict__ res,
@@ -254,14 +292,14 @@ __global__ __launch_bounds__(1024) void rms_fwd_long_kernel(
 // all rows of its block, so dgamma's partial sums stay in registers; the
 // blocks' partials are added by rms_dgamma_kernel in a fixed order.
 // ---------------------------------------------------------------------------
-template <typename T, int VEC, int TPR, int NV, bool DSUM>
+template <typename T, int VEC, int TPR, int NV, bool LOOSE, bool DSUM>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
     const T* __restrict__ dy, const T* __restrict__ dsum,
     const T* __restrict__ h, const float* __restrict__ gamma,
     const float* __restrict__ rstd, T* __restrict__ dx,
     float* __restrict__ partial, long rows, int C) {
-  using VecT = T __attribute__((ext_vector_type(VEC)));
-  using VecG = float __attribute__((ext_vector_type(VEC)));
+  using VecT = Vec<T, VEC>;
+  using VecG = Vec<float, VEC>;
   constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
   __shared__ float red[TPR > 64 ? TPR / 64 : 1];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -280,10 +318,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
       if (c < C) {
-        na[i] = __builtin_nontemporal_load((const VecT*)(dy + base + c));
-        nb[i] = *(const VecT*)(h + base + c);
+        na[i] = load_vec<VEC, LOOSE, true>(dy + base + c, C - c);
+        nb[i] = load_vec<VEC, LOOSE>(h + base + c, C - c);
         if constexpr (DSUM && AHEAD)
-          ne[i] = __builtin_nontemporal_load((const VecT*)(dsum + base + c));
+          ne[i] = load_vec<VEC, LOOSE, true>(dsum + base + c, C - c);
       }
     }
   };
@@ -305,7 +343,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
       if (c < C) {
-        const VecG g = *(const VecG*)(gamma + c);
+        const VecG g = load_vec<VEC, LOOSE>(gamma + c, C - c);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float d = (float)a[i][j], n = (float)b[i][j] * r;
@@ -317,7 +355,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
     m = row_sum_f32<TPR>(m, red) / C;
     // (without this the compiler keeps the row's products for the loop below,
     // in scratch memory where the registers do not hold them: 32768 columns)
-    if constexpr (!AHEAD && VEC > 1) {
+    if constexpr (!AHEAD) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         asm volatile("" : "+v"(*(int4_t*)&a[i]), "+v"(*(int4_t*)&b[i]));
@@ -326,9 +364,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * VEC;
       if (c < C) {
-        const VecG g = *(const VecG*)(gamma + c);
+        const VecG g = load_vec<VEC, LOOSE>(gamma + c, C - c);
         if constexpr (DSUM && !AHEAD)
-          e[i] = __builtin_nontemporal_load((const VecT*)(dsum + base + c));
+          e[i] = load_vec<VEC, LOOSE, true>(dsum + base + c, C - c);
         VecT o;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -336,7 +374,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
           if constexpr (DSUM) v += (float)e[i][j];
           o[j] = (T)v;
         }
-        *(VecT*)(dx + base + c) = o;
+        store_vec<VEC, LOOSE>(dx + base + c, C - c, o);
       }
     }
   }
@@ -347,7 +385,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
       if (c < C)
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          partial[(long)blockIdx.x * C + c + j] = dg[i][j];
+          if (!LOOSE || c + j < C)
+            partial[(long)blockIdx.x * C + c + j] = dg[i][j];
     }
   } else {
     __shared__ float part[RPB][TPR * NV * VEC];
@@ -437,60 +476,55 @@ __global__ __launch_bounds__(1024) void rms_dgamma_kernel(
 // ---------------------------------------------------------------------------
 struct RowPlan {
   int tpr = 0, nv = 0;  // 0: the kernel that reads the row again
-  bool vec = false;     // 16-byte accesses
+  bool loose = false;   // rows that are not whole, aligned vectors
 };
 
 RowPlan plan_rows(long rows, int C, size_t size, bool aligned) {
   RowPlan p;
-  const int vec = aligned && (C * size) % 16 == 0 ? (int)(16 / size) : 1;
-  p.vec = vec > 1;
+  const int vec = (int)(16 / size);
+  p.loose = !aligned || C % vec;
   auto fits = [&](int tpr, int nv) {
     if (p.tpr == 0 && C <= (long)tpr * nv * vec) {
       p.tpr = tpr;
       p.nv = nv;
     }
   };
-  if (p.vec) {
-    if (rows >= 1024 || C <= 64 * vec) {
-      fits(64, 1);
-      fits(64, 2);
-      fits(64, 4);
-    }
-    fits(256, 1);
-    fits(256, 2);
-    fits(256, 4);
-    fits(1024, 2);
-    fits(1024, 4);
-  } else {
+  if (rows >= 1024 || C <= 64 * vec) {
+    fits(64, 1);
+    fits(64, 2);
     fits(64, 4);
-    fits(256, 4);
-    fits(256, 16);
-    fits(1024, 16);
   }
+  fits(256, 1);
+  fits(256, 2);
+  fits(256, 4);
+  fits(1024, 2);
+  fits(1024, 4);
   return p;
 }
 
-#define RMS_CASE(VEC_, TPR_, NV_) \
-  if (p.vec == (VEC_ > 1) && p.tpr == TPR_ && p.nv == NV_) { \
-    constexpr int VEC = VEC_, TPR = TPR_, NV = NV_; \
-    LAUNCH(); \
+#define RMS_CASE(TPR_, NV_) \
+  if (p.tpr == TPR_ && p.nv == NV_) { \
+    constexpr int TPR = TPR_, NV = NV_; \
+    if (p.loose) { \
+      constexpr bool LOOSE = true; \
+      LAUNCH(); \
+    } else { \
+      constexpr bool LOOSE = false; \
+      LAUNCH(); \
+    } \
     return; \
   }
 
-// LAUNCH sees VEC, TPR and NV as constants
-#define RMS_DISPATCH(FULL) \
-  RMS_CASE(FULL, 64, 1) \
-  RMS_CASE(FULL, 64, 2) \
-  RMS_CASE(FULL, 64, 4) \
-  RMS_CASE(FULL, 256, 1) \
-  RMS_CASE(FULL, 256, 2) \
-  RMS_CASE(FULL, 256, 4) \
-  RMS_CASE(FULL, 1024, 2) \
-  RMS_CASE(FULL, 1024, 4) \
-  RMS_CASE(1, 64, 4) \
-  RMS_CASE(1, 256, 4) \
-  RMS_CASE(1, 256, 16) \
-  RMS_CASE(1, 1024, 16)
+// LAUNCH sees VEC, TPR, NV and LOOSE as constants
+#define RMS_DISPATCH() \
+  RMS_CASE(64, 1) \
+  RMS_CASE(64, 2) \
+  RMS_CASE(64, 4) \
+  RMS_CASE(256, 1) \
+  RMS_CASE(256, 2) \
+  RMS_CASE(256, 4) \
+  RMS_CASE(1024, 2) \
+  RMS_CASE(1024, 4)
 
 bool aligned16(std::initializer_list<const void*> ps) {
   for (auto p : ps)
@@ -519,11 +553,12 @@ void fwd_launch(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
   T* yp = INT8 ? nullptr : (T*)y.ptr;
   signed char* qp = INT8 ? (signed char*)y.ptr : nullptr;
   // a launch has fewer than 2^32 threads: 2^21 blocks of 1024 at most
+  constexpr int VEC = 16 / sizeof(T);
 #define LAUNCH()                                                            \
   constexpr int RPB = TPR < 256 ? 256 / TPR : 1;                            \
   for (long r0 = 0; r0 < rows; r0 += (1L << 21) * RPB) {                    \
     const long n = std::min(rows - r0, (1L << 21) * RPB), at = r0 * C;      \
-    rms_fwd_kernel<T, VEC, TPR, NV, RES, INT8>                              \
+    rms_fwd_kernel<T, VEC, TPR, NV, LOOSE, RES, INT8>                       \
         <<<(unsigned)((n + RPB - 1) / RPB), TPR < 256 ? 256 : TPR, 0,       \
            lc.stream>>>(                                                    \
             x.data<T>() + at, RES ? res.data<T>() + at : nullptr,           \
@@ -533,7 +568,7 @@ void fwd_launch(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
             RES ? sum.data<T>() + at : nullptr,                             \
             rstd.defined() ? rstd.data<float>() + r0 : nullptr, n, C, eps); \
   }
-  RMS_DISPATCH((int)(16 / sizeof(T)))
+  RMS_DISPATCH()
 #undef LAUNCH
   rms_fwd_long_kernel<T, RES, INT8>
       <<<(unsigned)std::min<long>(rows, 4096), 1024, 0, lc.stream>>>(
@@ -551,12 +586,13 @@ void bwd_launch(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
   RowPlan p = plan_rows(rows, C, sizeof(T),
                         aligned16({dy.ptr, dsum.ptr, h.ptr, gamma.ptr,
                                    dx.ptr}));
+  constexpr int VEC = 16 / sizeof(T);
 #define LAUNCH()                                                          \
-  rms_bwd_kernel<T, VEC, TPR, NV, DSUM>                                   \
+  rms_bwd_kernel<T, VEC, TPR, NV, LOOSE, DSUM>                            \
       <<<(unsigned)nblk, TPR < 256 ? 256 : TPR, 0, lc.stream>>>(          \
           dy.data<T>(), dsum.data<T>(), h.data<T>(), gamma.data<float>(), \
           rstd.data<float>(), dx.data<T>(), partial, rows, C)
-  RMS_DISPATCH((int)(16 / sizeof(T)))
+  RMS_DISPATCH()
 #undef LAUNCH
   rms_bwd_long_kernel<T, DSUM>
       <<<(unsigned)std::min<long>(rows, 4096), 1024, 0, lc.stream>>>(
