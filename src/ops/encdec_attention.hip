@@ -26,6 +26,7 @@
 //
 // Measured at 4x16 heads, 1024 over 2048 keys, all of them kept, bf16:
 //   head size 64:   forward 61 us (560 TFLOP/s), backward 186 us (460)
+//   head size 96:   forward 79 us (650), backward 236 us (550)
 //   head size 128:  forward 101 us (680), backward 412 us (417)
 // and in fp32 at 2x16 heads, 1024 over 1024 keys of 64: 83 us (104), 270 us
 // (79).  A large library product reaches 1198 in bf16, 154 in fp32.  Long
@@ -73,12 +74,15 @@ template <> struct Mat<float> {
   }
 };
 
-// Waves a SIMD: two where a wave's registers (256 then) hold the `n` operands
-// of a row and its accumulators, which hides most of each wave's latencies
-// behind the other; else one.  32-bit fragments take twice the room.
+// Waves a SIMD: two where the `n` operands of a row take at most `most` bytes,
+// so that a wave's 256 registers hold them and their accumulators; else one.
+// The second hides most of the first's latencies: dK and dV of size 96 in 16
+// bits are faster with two, of which 12 registers lie in scratch memory, than
+// with one (backward of 4x16 heads, 1024 over 2048 keys: 236 us, 332); of size
+// 128, where 59 would, with one (412 us, 527).
 template <typename T, int DP>
-constexpr int waves(int n) {
-  return n * DP * (int)sizeof(T) <= 256 ? 2 : 1;
+constexpr int waves(int n, int most = 256) {
+  return n * DP * (int)sizeof(T) <= most ? 2 : 1;
 }
 
 // one [B, S, heads, D] view: strides in elements, D contiguous
@@ -102,7 +106,8 @@ struct Att {
 };
 
 // ---------------------------------------------------------------------------
-// LDS tiles [rows][DP] in 16-byte chunks.  The chunk's place in its row is
+// LDS tiles [rows][DP] in 16-byte chunks (rows of 96 lie as those of 128, whose
+// last quarter nobody reads).  The chunk's place in its row is
 // XORed with a function of the row, chosen so that both readers are free of
 // bank conflicts: 16 rows at one chunk (row fragments), and 4 rows at 4
 // neighbouring chunks (the transposing read).
@@ -110,8 +115,9 @@ struct Att {
 template <typename T, int DP>
 struct Tile {
   static constexpr int EPC = 16 / sizeof(T);  // elements a chunk
-  static constexpr int CPR = DP / EPC;        // chunks a row
-  static constexpr int RB = DP * (int)sizeof(T);
+  static constexpr int WIDE = DP == 96 ? 128 : DP;
+  static constexpr int CPR = WIDE / EPC;      // chunks a row
+  static constexpr int RB = WIDE * (int)sizeof(T);
   static DEV_INLINE int swz(int row) {
     if constexpr (RB == 64) return (row >> 2) & 3;
     if constexpr (RB == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
@@ -574,7 +580,7 @@ DEV_INLINE void finish_row(const Att& a, const float16_t (&acc)[DP / 32],
 // half the keys each (58), a raised wave priority for the products (55).
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int NW, int BN>
-__global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_fwd_kernel(Att a) {
+__global__ __launch_bounds__(NW * 64, (waves<T, DP>(1, 384))) void att_fwd_kernel(Att a) {
   using TL = Tile<T, DP>;
   constexpr int NT = NW * 64, KB = BN / 32, BYTES = BN * TL::RB;
   __shared__ __attribute__((aligned(16))) char lk[2][BYTES], lv[2][BYTES];
@@ -859,7 +865,7 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
 // rows is read from LDS as rows and as columns, 16 KB for 32x32 scores, so LDS
 // is busy as long as the matrix cores.
 template <typename T, int DP, int NW, int BM>
-__global__ __launch_bounds__(NW * 64, (waves<T, DP>(2))) void att_dkv_kernel(Att a) {
+__global__ __launch_bounds__(NW * 64, (waves<T, DP>(2, 384))) void att_dkv_kernel(Att a) {
   using TL = Tile<T, DP>;
   constexpr int NT = NW * 64, BYTES = BM * TL::RB;
   __shared__ __attribute__((aligned(16))) char lq[2][BYTES], lg[2][BYTES];
@@ -1042,7 +1048,7 @@ __global__ __launch_bounds__(256) void att_dkv_join_kernel(Att a, int DP) {
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-int pad_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+int pad_dim(int D) { return (D + 31) / 32 * 32; }
 
 // As many splits as bring the launch to `want` blocks, none shorter than
 // `least` tiles of 64
@@ -1171,6 +1177,7 @@ template <typename F>
 void by_dim(int DP, F f) {
   if (DP == 32) f(std::integral_constant<int, 32>{});
   else if (DP == 64) f(std::integral_constant<int, 64>{});
+  else if (DP == 96) f(std::integral_constant<int, 96>{});
   else f(std::integral_constant<int, 128>{});
 }
 

@@ -411,3 +411,14 @@ def test_more_refusals_on_the_gpu():
     dq, = autograd.grad([o], [nd(q)], create_graph=True, retain_graph=True)
     with pytest.raises(RuntimeError):  # no second derivatives
         dq.to_torch().square().sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('size', [(2, 4, 2, 40, 100, 96), (1, 2, 1, 1, 700, 72),
+                                  (1, 3, 3, 200, 65, 80), (1, 4, 2, 9, 3000, 95)])
+def test_head_sizes_of_65_to_96(size, dtype):
+    for layout in ('NTC', 'TNC'):
+        d = make(size, dtype, 'cuda:0', layout, seed=11, mask=True,
+                 lengths=[size[4], size[4] // 2][:size[0]])
+        check(call(d, size, layout, grad=True), oracle(d, size, layout))
