@@ -127,8 +127,6 @@ def _encdec_native(queries, keys_values, values, heads, kv_heads,
         raise ValueError(f'encdec_attention: layout must be NTC or TNC, got '
                          f'{layout!r}')
     heads = int(heads)
-    if valid_length is not None and str(valid_length.dtype) == 'int64':
-        valid_length = valid_length.astype('int32')
     more = [values, valid_length, mask]
     attrs = {'heads': str(heads),
              'kv_heads': str(heads if kv_heads is None else int(kv_heads)),

@@ -202,9 +202,10 @@ void EncDecInfer(const NodeAttrs& a, const std::vector<TShape>& is,
                       e.values.dtype == e.kv.dtype),
            "encdec_attention: the values must be like the keys");
   MX_CHECK(!a.GetBool("has_length", false) ||
-               (e.len.shape == TShape{e.B} && e.len.dtype == kInt32),
-           "encdec_attention: valid_length must hold one int32 for each "
-           "sequence");
+               (e.len.shape == TShape{e.B} &&
+                (e.len.dtype == kInt32 || e.len.dtype == kInt64)),
+           "encdec_attention: valid_length must hold one int32 or int64 for "
+           "each sequence");
   MX_CHECK(!a.GetBool("has_mask", false) ||
                (e.mask.shape == TShape{e.B, e.sk} &&
                 (e.mask.dtype == kUint8 || e.mask.dtype == kBool)),
@@ -226,7 +227,10 @@ struct Walk {
     return row(e.kv, b, s) + h * e.D * (e.values.defined() ? 1 : 2);
   }
   bool keep(int64_t b, int64_t s) const {
-    if (e.len.defined() && s >= e.len.data<int>()[b]) return false;
+    if (e.len.defined() &&
+        s >= (e.len.dtype == kInt64 ? e.len.data<int64_t>()[b]
+                                    : e.len.data<int>()[b]))
+      return false;
     return !e.mask.defined() || e.mask.data<uint8_t>()[b * e.sk + s];
   }
   // weights of one row; false if it has no key

@@ -93,7 +93,7 @@ struct View {
 
 struct Att {
   View q, k, v, o, dout, dq, dk, dv;
-  const int* len;        // [B] or null
+  const void* len;       // [B] int32 or (len64) int64, or null
   const uint8_t* mask;   // [B, Sk], 0: masked, or null
   float* lse;            // [B, H, Sq] log2 of the row's sum, +inf: no key
   float* delta;          // [B, H, Sq]
@@ -101,6 +101,7 @@ struct Att {
   int B, H, Hk, G, Sq, Sk, D;
   int nsplit;
   int vec;               // 16-byte accesses
+  bool len64;
   float scale;           // 1 / sqrt(D)
   float inv_sq;          // 1 / Sq
 };
@@ -257,9 +258,9 @@ DEV_INLINE float pair_sum(float v) {
 }
 
 DEV_INLINE int kept_keys(const Att& a, int b) {
-  int n = a.Sk;
-  if (a.len) n = min(n, max(0, a.len[b]));
-  return n;
+  if (!a.len) return a.Sk;
+  const long n = a.len64 ? ((const long*)a.len)[b] : ((const int*)a.len)[b];
+  return (int)min((long)a.Sk, max(0L, n));
 }
 
 // The sequence and key head of the i-th of B * Hk.  Neighbours are sequences,
@@ -1124,8 +1125,10 @@ Att make_att(const Arr& q, const Arr& kv, const Arr& values, int heads,
                  values.dtype == kv.dtype,
              name << ": the values must be like the keys");
   }
-  MX_CHECK(!len.defined() || (len.dtype == kInt32 && len.numel() == hq.B),
-           name << ": valid_length must hold one int32 for each sequence");
+  MX_CHECK(!len.defined() || ((len.dtype == kInt32 || len.dtype == kInt64) &&
+                              len.numel() == hq.B),
+           name << ": valid_length must hold one int32 or int64 for each "
+                   "sequence");
   MX_CHECK(!mask.defined() || ((mask.dtype == kUint8 || mask.dtype == kBool) &&
                                mask.numel() == hk.B * hk.S),
            name << ": the mask must hold one byte for each key");
@@ -1143,7 +1146,8 @@ Att make_att(const Arr& q, const Arr& kv, const Arr& values, int heads,
     a.k = view(kv, hk, 0, 2 * D);
     a.v = view(kv, hk, D, 2 * D);
   }
-  a.len = len.data<int>();
+  a.len = len.ptr;
+  a.len64 = len.dtype == kInt64;
   a.mask = mask.data<uint8_t>();
   a.B = (int)hq.B;
   a.H = heads;

@@ -86,8 +86,8 @@ void rms_norm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
 
 // ---- encdec_attention.hip -------------------------------------------------
 // q [B,Sq,heads*D] over kv [B,Sk,kv_heads*2*D] (a head's key, then its value;
-// or keys and values apart), tnc: [S,B,..].  len int32 [B], mask byte [B,Sk],
-// lse fp32 [B,heads,Sq] (optional), work: fp32 of the sizes that
+// or keys and values apart), tnc: [S,B,..].  len int32 or int64 [B], mask byte
+// [B,Sk], lse fp32 [B,heads,Sq] (optional), work: fp32 of the sizes that
 // encdec_attention_workspace gives, {forward, backward}
 std::vector<int64_t> encdec_attention_workspace(int64_t B, int64_t H,
                                                 int64_t Hk, int64_t Sq,

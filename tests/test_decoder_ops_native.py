@@ -390,3 +390,31 @@ def test_both_frontends_run_one_kernel(native, dtype):
     same(gn.grad, gg)
     same(tn, t)
     set_native(True)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('sq', [1, 40])
+def test_lengths_that_int32_does_not_hold(native, sq, device):
+    """int64 lengths mean what the same lengths within the keys mean, also
+    where neither int32 nor float32 holds them."""
+    rs = np.random.RandomState(13)
+    far = [(1 << 40), (1 << 63) - 1, -(1 << 40), (1 << 32) + 2, 1 << 31,
+           -(1 << 63), 4]
+    near_by = [9, 9, 0, 9, 9, 0, 4]
+    q, dout = (rs.randn(7, sq, 16).astype('float32') for _ in range(2))
+    kv = rs.randn(7, 9, 16).astype('float32')
+    got = []
+    for length, dtype in ((far, 'int64'), (near_by, 'int64'),
+                          (near_by, 'int32')):
+        ins = [arr(q, device), arr(kv, device)]
+        for v in ins:
+            v.attach_grad()
+        with autograd.record():
+            out = mx.nd.contrib.encdec_attention(
+                *ins, heads=2, kv_heads=1,
+                valid_length=arr(np.array(length, dtype), device))
+        autograd.backward([out], [arr(dout, device)])
+        got.append([t.asnumpy() for t in [out] + [v.grad for v in ins]])
+    for a, b, c in zip(*got):
+        assert np.array_equal(a, c) and np.array_equal(b, c)
+    assert np.abs(got[0][0]).max((1, 2))[[0, 1, 3, 4, 6]].all()
