@@ -156,12 +156,36 @@ __global__ void bin_param_kernel(const T* __restrict__ a,
     y[i] = stf<T>(OP::f(ldf(a[i]), ldf(b[i]), alpha, beta));
 }
 
+// Only the 16-bit types go through float32: whole numbers, and float64, it
+// does not hold.
+template <typename TD, typename TS>
+HD TD cast_value(TS v) {
+  constexpr bool half = (std::is_same<TS, _Float16>::value ||
+                         std::is_same<TS, __bf16>::value ||
+                         std::is_same<TD, _Float16>::value ||
+                         std::is_same<TD, __bf16>::value);
+  if constexpr (half) return (TD)(float)v;
+  else return (TD)v;
+}
+
+// MXC_DISPATCH_ALL, and the types that only a cast reads and writes
+#define DISPATCH_CAST(DTYPE, NAME, ...)   \
+  if ((DTYPE) == kFloat64) {              \
+    using scalar_t = double;              \
+    __VA_ARGS__                           \
+  } else if ((DTYPE) == kInt8) {          \
+    using scalar_t = signed char;         \
+    __VA_ARGS__                           \
+  } else {                                \
+    MXC_DISPATCH_ALL(DTYPE, NAME, __VA_ARGS__) \
+  }
+
 template <typename TS, typename TD>
 __global__ void cast_kernel(const TS* __restrict__ x, TD* __restrict__ y,
                             long n) {
   for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n;
        i += (long)gridDim.x * blockDim.x)
-    y[i] = (TD)(float)x[i];
+    y[i] = cast_value<TD>(x[i]);
 }
 
 template <typename T>
@@ -749,9 +773,9 @@ bool _registered = [] {
               const std::vector<TBlob>& out) {
         long n = out[0].size();
         if (n == 0) return;
-        MXC_DISPATCH_ALL(in[0].dtype, "cast_src", {
+        DISPATCH_CAST(in[0].dtype, "cast_src", {
           using src_t = scalar_t;
-          MXC_DISPATCH_ALL(out[0].dtype, "cast_dst", {
+          DISPATCH_CAST(out[0].dtype, "cast_dst", {
             cast_kernel<src_t, scalar_t><<<grid_for(n), kBlock, 0,
                                            o.rc.stream>>>(
                 (const src_t*)in[0].dptr, (scalar_t*)out[0].dptr, n);
@@ -762,12 +786,12 @@ bool _registered = [] {
       .cpu([](const NodeAttrs&, const OpCtx&, const std::vector<TBlob>& in,
               const std::vector<TBlob>& out) {
         long n = out[0].size();
-        MXC_DISPATCH_ALL(in[0].dtype, "cast_src", {
+        DISPATCH_CAST(in[0].dtype, "cast_src", {
           using src_t = scalar_t;
           auto* x = (const src_t*)in[0].dptr;
-          MXC_DISPATCH_ALL(out[0].dtype, "cast_dst", {
+          DISPATCH_CAST(out[0].dtype, "cast_dst", {
             auto* y = (scalar_t*)out[0].dptr;
-            for (long i = 0; i < n; ++i) y[i] = (scalar_t)(float)x[i];
+            for (long i = 0; i < n; ++i) y[i] = cast_value<scalar_t>(x[i]);
           });
         });
       })
