@@ -177,7 +177,11 @@ def _sample_native(logits, uniform, temperature, top_k, top_p, min_p,
             ('top_p', top_p, 'float32', 0.0, 1.0),
             ('min_p', min_p, 'float32', 0.0, 1.0)):
         if isinstance(value, NDArray):
-            ins.append(value if str(value.dtype) == dtype
+            have = str(value.dtype)
+            if ('float' in have) != ('float' in dtype):
+                raise TypeError(f'sample_tokens: {name} of {have}')
+            # (int64 as it is: int32 may not hold it)
+            ins.append(value if have == dtype or have == 'int64'
                        else value.astype(dtype))
             attrs['has_' + name] = '1'
         else:

@@ -364,7 +364,9 @@ void SampleCpu(const NodeAttrs& a, const OpCtx&, V in, V out) {
     }
     const double t = s.t.defined() ? s.t.data<float>()[n]
                                    : a.GetFloat("temperature", 1);
-    int64_t k = s.k.defined() ? s.k.data<int>()[n] : a.GetInt("top_k", 0);
+    int64_t k = !s.k.defined()        ? a.GetInt("top_k", 0)
+                : s.k.dtype == kInt64 ? s.k.data<int64_t>()[n]
+                                      : s.k.data<int>()[n];
     const double p = s.p.defined() ? s.p.data<float>()[n]
                                    : a.GetFloat("top_p", 1);
     const double m = s.m.defined() ? s.m.data<float>()[n]
@@ -511,7 +513,8 @@ bool _registered = [] {
       for (const char* p : {"temperature", "top_k", "top_p", "min_p"})
         if (a.GetBool(std::string("has_") + p, false)) {
           MX_CHECK(i < is.size() && is[i] == n &&
-                       it[i] == (p[4] == 'k' ? kInt32 : kFloat32),
+                       (p[4] == 'k' ? it[i] == kInt32 || it[i] == kInt64
+                                    : it[i] == kFloat32),
                    "sample_tokens: " << p << " must hold one value a row");
           ++i;
         }

@@ -47,7 +47,8 @@ struct Sample {
   const float* u;
   // one a row where the pointer is given, else the value
   const float *tp, *pp, *mp;
-  const int* kp;
+  const void* kp;  // int32 or (k64) int64
+  bool k64;
   double t, p, m;
   int k;
   int sbits;
@@ -264,8 +265,11 @@ DEV_INLINE void count_row(const Sample& a, const T* x, long i0, long i1,
 
 // how many the row may keep; 0: all.  The numbers are counted only for this
 DEV_INLINE int number_kept(const Sample& a, int n, const Row& r) {
-  const int k = r.greedy ? 1 : a.kp ? a.kp[n] : a.k;
-  return k > 0 && k < a.V ? k : 0;
+  const long k = r.greedy ? 1
+                 : !a.kp  ? a.k
+                 : a.k64  ? ((const long*)a.kp)[n]
+                          : ((const int*)a.kp)[n];
+  return k > 0 && k < a.V ? (int)k : 0;
 }
 
 template <typename T>
@@ -835,8 +839,10 @@ void sample_tokens_raw(const LaunchCtx& lc, const Arr& logits, const Arr& u,
   for (const Arr* x : {&temperature, &top_p, &min_p})
     MX_CHECK(!x->defined() || (x->dtype == kFloat32 && x->numel() == N),
              "sample_tokens: parameters are one number, or a float32 a row");
-  MX_CHECK(!top_k.defined() || (top_k.dtype == kInt32 && top_k.numel() == N),
-           "sample_tokens: top_k is one number, or an int32 a row");
+  MX_CHECK(!top_k.defined() ||
+               ((top_k.dtype == kInt32 || top_k.dtype == kInt64) &&
+                top_k.numel() == N),
+           "sample_tokens: top_k is one number, or an int32 or int64 a row");
   MX_CHECK((work.defined() ? work.numel() * (int64_t)dtype_size(work.dtype)
                            : 0) >= sample_tokens_workspace(N, V),
            "sample_tokens: workspace too small");
@@ -849,7 +855,8 @@ void sample_tokens_raw(const LaunchCtx& lc, const Arr& logits, const Arr& u,
   a.tp = temperature.data<float>();
   a.pp = top_p.data<float>();
   a.mp = min_p.data<float>();
-  a.kp = top_k.data<int>();
+  a.kp = top_k.ptr;
+  a.k64 = top_k.dtype == kInt64;
   a.t = t;
   a.p = p;
   a.m = m;

@@ -418,3 +418,31 @@ def test_lengths_that_int32_does_not_hold(native, sq, device):
     for a, b, c in zip(*got):
         assert np.array_equal(a, c) and np.array_equal(b, c)
     assert np.abs(got[0][0]).max((1, 2))[[0, 1, 3, 4, 6]].all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_types_of_sampling_parameters(native, device):
+    """The torch frontend's rules: parameters of the wrong kind are refused,
+    the others' values count, whatever their size."""
+    rs = np.random.RandomState(14)
+    x, u = arr(rs.randn(6, 30).astype('float32'), device), \
+        arr(rs.rand(6).astype('float32'), device)
+    f = mx.nd.contrib.sample_tokens
+    with pytest.raises(TypeError):
+        f(x, u, top_k=arr(np.full(6, 1.9, 'float32'), device))
+    for name in ('temperature', 'top_p', 'min_p'):
+        with pytest.raises(TypeError):
+            f(x, u, **{name: arr(np.ones(6, 'int32'), device)})
+    want = f(x, u, top_k=arr(np.array([0, 1, 5, 0, 30, 0], 'int32'), device))
+    # (of no limit, 1, 5, no limit, as many as there are and less than none)
+    far = np.array([1 << 32, 1, 5, (1 << 63) - 1, 30, -(1 << 40)], 'int64')
+    assert np.array_equal(f(x, u, top_k=arr(far, device)).asnumpy(),
+                          want.asnumpy())
+    for kind in ('int8', 'uint8', 'int64'):
+        got = f(x, u, top_k=arr(np.array([0, 1, 5, 0, 30, 0], kind), device))
+        assert np.array_equal(got.asnumpy(), want.asnumpy())
+    t = np.array([0.5, 1, 0, 2, 1, 0.25])
+    want = f(x, u, temperature=arr(t.astype('float32'), device))
+    for kind in ('float16', 'float64'):
+        got = f(x, u, temperature=arr(t.astype(kind), device))
+        assert np.array_equal(got.asnumpy(), want.asnumpy())
