@@ -208,8 +208,9 @@ DEV_INLINE double temperature(const Sample& a, int n) {
 DEV_INLINE Row make_row(double temp, float top) {
   Row r;
   r.greedy = !(temp > 0.0);
-  r.inv = r.greedy ? 1e300 : 1.0 / temp;
-  r.scale = r.greedy ? 1e300 : r.inv * (STEP * 1.4426950408889634);
+  // finite, so that the maximum itself lies no way below it, whatever T
+  r.inv = r.greedy ? 1e300 : fmin(1.0 / temp, 1e300);
+  r.scale = r.inv * (STEP * 1.4426950408889634);
   r.top = top == kInf ? 0x1p129 : (double)top;
   r.ftop = top;
   return r;

@@ -294,3 +294,19 @@ def test_graphs_of_long_rows():
             e = mx.nd.contrib.sample_tokens(nd(v), nd(u), **kw)
             for a, b in zip(o, e):
                 assert np.array_equal(a.asnumpy(), b.asnumpy())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('v', [300, 70001])
+@pytest.mark.parametrize('temperature', [5e-324, 1e-310, 1e-307, 1e-300])
+def test_smallest_temperatures(temperature, v, device):
+    """Whose reciprocal float64 does not hold: the largest logit, and one of
+    those where several are equal."""
+    x, u = make(4, v, torch.float32, device, seed=7)
+    x[1, ::3] = 9.5
+    x[2] = 0.0
+    x[3, 5] = math.inf
+    for kw in ({}, dict(top_k=7, top_p=0.5), dict(min_p=0.5)):
+        check(x, u, temperature=temperature, **kw)
+    rows = torch.tensor([1e-45, 1e-40, 1e-38, 0.0], device=device)
+    check(x, u, temperature=rows)
