@@ -149,7 +149,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0,
     largest weight; the token is the first whose running sum exceeds uniform
     times the kept sum.  A temperature of 0 takes the largest logit.  Each
     parameter is a number, or an array of one for each row (float32, top_k
-    int32; there a temperature that is not positive counts as 0).  A NaN is
+    int32), whose values count as the nearest of the parameter's range:
+    temperature 0 to 1e30, top_k from 0 on, top_p and min_p 0 to 1.  A NaN is
     never drawn; a row without a finite or infinite logit gives -1.
 
     Returns int32 tokens (N,), or with ``get_prob`` ``[tokens, logp]``: the

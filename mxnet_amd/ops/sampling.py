@@ -86,6 +86,7 @@ def _plain(logits, uniform, temperature, top_k, top_p, min_p, get_prob):
         return t.double()[:, None]
 
     temp, k, p, m = (col(x) for x in (temperature, top_k, top_p, min_p))
+    temp, m = temp.clamp(max=1e30), m.clamp(max=1.0)
     if not n:
         return (torch.zeros(0, dtype=torch.int32, device=logits.device),
                 torch.zeros(0, device=logits.device) if get_prob else None)

@@ -362,14 +362,15 @@ void SampleCpu(const NodeAttrs& a, const OpCtx&, V in, V out) {
       *logp = std::numeric_limits<float>::quiet_NaN();
       continue;
     }
-    const double t = s.t.defined() ? s.t.data<float>()[n]
-                                   : a.GetFloat("temperature", 1);
+    const double t = s.t.defined()
+                         ? std::min<double>(s.t.data<float>()[n], 1e30)
+                         : a.GetFloat("temperature", 1);
     int64_t k = !s.k.defined()        ? a.GetInt("top_k", 0)
                 : s.k.dtype == kInt64 ? s.k.data<int64_t>()[n]
                                       : s.k.data<int>()[n];
     const double p = s.p.defined() ? s.p.data<float>()[n]
                                    : a.GetFloat("top_p", 1);
-    const double m = s.m.defined() ? s.m.data<float>()[n]
+    const double m = s.m.defined() ? std::min<double>(s.m.data<float>()[n], 1)
                                    : a.GetFloat("min_p", 0);
     if (!(t > 0)) k = 1;
     int64_t keep = k > 0 && k < V_ ? k : V_;

@@ -202,7 +202,9 @@ DEV_INLINE float entry_logit(u64 e) {
 }
 
 DEV_INLINE double temperature(const Sample& a, int n) {
-  return a.tp ? (double)a.tp[n] : a.t;
+  if (!a.tp) return a.t;
+  const double t = (double)a.tp[n];
+  return t > 1e30 ? 1e30 : t;
 }
 
 DEV_INLINE Row make_row(double temp, float top) {

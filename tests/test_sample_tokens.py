@@ -310,3 +310,31 @@ def test_smallest_temperatures(temperature, v, device):
         check(x, u, temperature=temperature, **kw)
     rows = torch.tensor([1e-45, 1e-40, 1e-38, 0.0], device=device)
     check(x, u, temperature=rows)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('v', [300, 70001])
+def test_parameters_of_rows_outside_their_range(v, device):
+    """Count as the nearest that lies in it, on the GPU as on the CPU."""
+    x, u = make(6, v, torch.float32, device, seed=8)
+    x[0, ::2] = -math.inf
+    x[1, ::5] = math.inf
+    x[2, ::3] = 9.5
+    x[4, 1:] = -math.inf
+    f = mx.nd.contrib.sample_tokens
+
+    def rows(value, dtype=torch.float32):
+        return nd(torch.full((6,), value, dtype=dtype, device=device))
+
+    for name, value, near in (('temperature', math.inf, 1e30),
+                              ('temperature', 3e38, 1e30),
+                              ('temperature', -1.0, 0.0),
+                              ('top_p', 1.5, 1.0), ('top_p', -1.0, 0.0),
+                              ('min_p', 2.0, 1.0), ('min_p', -1.0, 0.0)):
+        got = f(nd(x), nd(u), get_prob=True, **{name: rows(value)})
+        want = f(nd(x), nd(u), get_prob=True, **{name: near})
+        for g, w in zip(got, want):
+            assert np.array_equal(g.asnumpy(), w.asnumpy()), (name, value)
+        check(x, u, **{name: near})
+    got = f(nd(x), nd(u), top_k=rows(-3, torch.int32))
+    assert np.array_equal(got.asnumpy(), f(nd(x), nd(u)).asnumpy())
