@@ -153,7 +153,7 @@ std::vector<NDArray> RmsBwd(const TapeNode& n,
 struct EncDec {
   Arr q, kv, values, len, mask;
   int heads, kv_heads;
-  bool tnc;
+  bool apart, tnc;  // apart: values, also of no keys and without memory
   int64_t B, sq, sk, D;
 };
 
@@ -166,7 +166,8 @@ EncDec ReadEncDec(const NodeAttrs& a, const Arr* in, size_t n_in) {
   };
   e.q = next();
   e.kv = next();
-  if (a.GetBool("has_values", false)) e.values = next();
+  e.apart = a.GetBool("has_values", false);
+  if (e.apart) e.values = next();
   if (a.GetBool("has_length", false)) e.len = next();
   if (a.GetBool("has_mask", false)) e.mask = next();
   e.heads = (int)a.GetInt("heads", 1);
@@ -193,7 +194,7 @@ void EncDecInfer(const NodeAttrs& a, const std::vector<TShape>& is,
   std::vector<Arr> in;
   for (size_t i = 0; i < is.size(); ++i) in.emplace_back(nullptr, is[i], it[i]);
   const EncDec e = ReadEncDec(a, in.data(), in.size());
-  const bool apart = a.GetBool("has_values", false);
+  const bool apart = e.apart;
   MX_CHECK(IsFloat(e.q.dtype) && e.kv.dtype == e.q.dtype &&
                e.kv.size(2) == e.kv_heads * e.D * (apart ? 1 : 2) &&
                e.kv.size(e.tnc ? 1 : 0) == e.B,
@@ -224,7 +225,7 @@ struct Walk {
     return row(e.q, b, s) + h * e.D;
   }
   int64_t k(int64_t b, int64_t h, int64_t s) const {
-    return row(e.kv, b, s) + h * e.D * (e.values.defined() ? 1 : 2);
+    return row(e.kv, b, s) + h * e.D * (e.apart ? 1 : 2);
   }
   bool keep(int64_t b, int64_t s) const {
     if (e.len.defined() &&
@@ -259,8 +260,8 @@ void EncDecCpu(const NodeAttrs& a, const OpCtx&, V in, V out) {
   const auto ins = Arrs(in);
   const EncDec e = ReadEncDec(a, ins.data(), ins.size());
   const Walk w{e};
-  const float* vals = e.values.defined() ? e.values.data<float>()
-                                         : e.kv.data<float>() + e.D;
+  const float* vals = e.apart ? e.values.data<float>()
+                              : e.kv.data<float>() + e.D;
   std::vector<double> p(e.sk);
   for (int64_t b = 0; b < e.B; ++b)
     for (int64_t h = 0; h < e.heads; ++h)
@@ -284,7 +285,7 @@ void EncDecBwdCpu(const NodeAttrs& a, const OpCtx&, V in, V out) {
   const auto ins = Arrs(in, 3);
   const EncDec e = ReadEncDec(a, ins.data(), ins.size());
   const Walk w{e};
-  const bool apart = e.values.defined();
+  const bool apart = e.apart;
   const float* vals = apart ? e.values.data<float>()
                             : e.kv.data<float>() + e.D;
   const double c = 1 / std::sqrt((double)e.D);

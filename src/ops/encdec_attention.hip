@@ -1107,6 +1107,10 @@ View view(const Arr& x, const Heads& h, long off, long sh) {
   return View{(char*)x.ptr + off * dtype_size(x.dtype), h.sb, h.ss, sh};
 }
 
+// whether the values come apart from the keys (an array of no keys has no
+// memory, but axes)
+bool given(const Arr& values) { return values.dim() > 0; }
+
 Att make_att(const Arr& q, const Arr& kv, const Arr& values, int heads,
              int kv_heads, const Arr& len, const Arr& mask, bool tnc) {
   const char* name = "encdec_attention";
@@ -1115,11 +1119,12 @@ Att make_att(const Arr& q, const Arr& kv, const Arr& values, int heads,
            name << ": kv_heads must divide heads");
   MX_CHECK(q.size(2) % heads == 0, name << ": heads must divide the queries");
   const long D = q.size(2) / heads;
+  const bool apart = given(values);
   MX_CHECK(D >= 1 && D <= 128, name << ": head sizes of 1 to 128, got " << D);
   MX_CHECK(hq.B == hk.B && kv.dtype == q.dtype &&
-               kv.size(2) == kv_heads * D * (values.defined() ? 1 : 2),
+               kv.size(2) == kv_heads * D * (apart ? 1 : 2),
            name << ": the keys do not fit the queries and heads");
-  if (values.defined()) {
+  if (apart) {
     const Heads hv = lead(values, tnc, name);
     MX_CHECK(hv.B == hk.B && hv.S == hk.S && values.size(2) == kv.size(2) &&
                  values.dtype == kv.dtype,
@@ -1139,7 +1144,7 @@ Att make_att(const Arr& q, const Arr& kv, const Arr& values, int heads,
            name << ": too many rows, keys, heads or sequences");
   Att a = {};
   a.q = view(q, hq, 0, D);
-  if (values.defined()) {
+  if (apart) {
     a.k = view(kv, hk, 0, D);
     a.v = view(values, hk, 0, D);
   } else {
@@ -1300,8 +1305,8 @@ void encdec_attention_bwd_raw(const LaunchCtx& lc, const Arr& dout,
                out.shape == q.shape && out.dtype == q.dtype &&
                dq.shape == q.shape && dq.dtype == q.dtype &&
                dkv.shape == kv.shape && dkv.dtype == kv.dtype &&
-               values.defined() == dvalues.defined() &&
-               (!values.defined() || (dvalues.shape == values.shape &&
+               given(values) == given(dvalues) &&
+               (!given(values) || (dvalues.shape == values.shape &&
                                       dvalues.dtype == values.dtype)),
            "encdec_attention backward: a gradient must be like its input");
   const long rows = (long)a.B * a.H * a.Sq;
@@ -1315,7 +1320,7 @@ void encdec_attention_bwd_raw(const LaunchCtx& lc, const Arr& dout,
   a.dout = view(dout, lead(dout, tnc, "dout"), 0, a.D);
   a.dq = view(dq, lead(dq, tnc, "dq"), 0, a.D);
   const Heads hk = lead(dkv, tnc, "dkv");
-  if (values.defined()) {
+  if (given(values)) {
     a.dk = view(dkv, hk, 0, a.D);
     a.dv = view(dvalues, hk, 0, a.D);
   } else {

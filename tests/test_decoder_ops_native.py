@@ -446,3 +446,20 @@ def test_types_of_sampling_parameters(native, device):
     for kind in ('float16', 'float64'):
         got = f(x, u, temperature=arr(t.astype(kind), device))
         assert np.array_equal(got.asnumpy(), want.asnumpy())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('apart', [False, True])
+def test_attention_over_no_keys(native, apart, device):
+    q = np.ones((2, 3, 16), 'float32')
+    ins = [arr(q, device)] + [
+        mx.nd.zeros((2, 0, 8 if apart else 16), ctx=ctx(device))
+        for _ in range(2 if apart else 1)]
+    for v in ins:
+        v.attach_grad()
+    with autograd.record():
+        out = mx.nd.contrib.encdec_attention(*ins, heads=4, kv_heads=2)
+    autograd.backward([out], [arr(q, device)])
+    assert out.shape == q.shape and not out.asnumpy().any()
+    for v in ins:
+        assert v.grad.shape == v.shape and not v.grad.asnumpy().any()

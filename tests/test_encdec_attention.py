@@ -422,3 +422,16 @@ def test_head_sizes_of_65_to_96(size, dtype):
         d = make(size, dtype, 'cuda:0', layout, seed=11, mask=True,
                  lengths=[size[4], size[4] // 2][:size[0]])
         check(call(d, size, layout, grad=True), oracle(d, size, layout))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('layout', ['NTC', 'TNC'])
+@pytest.mark.parametrize('size', [(2, 2, 1, 0, 5, 8), (2, 2, 1, 3, 0, 8),
+                                  (2, 4, 4, 40, 0, 16), (0, 2, 1, 3, 5, 8)])
+def test_nothing_to_do_with_values_apart(size, layout, device):
+    """An array of no keys has no memory; its attention is zeros."""
+    for dtype in TYPES:
+        d = make(size, dtype, device, layout, apart=True)
+        got = call(d, size, layout, grad=True)
+        for g, name in zip(got, ('q', 'q', 'kv', 'values')):
+            assert g.shape == d[name].shape and not g.any()
