@@ -16,6 +16,7 @@ C-major rows), selected by Gluon layers via ``layout='NHWC'``.
 """
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from .dispatch import hip_required, use_hip
 
@@ -631,9 +632,15 @@ class _RMSNorm(torch.autograd.Function):
 
 
 def needs_grad(*tensors):
-    """Whether autograd has to see an operator of these (or None)."""
-    return torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in tensors)
+    """Whether autograd has to see an operator of these (or None): a backward
+    pass follows, or they carry a tangent (which the operators' autograd
+    functions refuse, and which would be lost beside them)."""
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None
+        for t in tensors)
 
 
 def _rms_norm_check(x, gamma, residual, out_type):

@@ -438,3 +438,37 @@ def test_captured_backward():
         torch.cuda.synchronize()
         for a, b in zip(caught, call()):
             assert torch.equal(a, b)
+
+
+def test_a_tangent_is_seen():
+    from mxnet_amd.ops.nn import needs_grad
+    x = torch.randn(3, 8)
+    assert not needs_grad(x, None)
+    with torch.autograd.forward_ad.dual_level():
+        assert not needs_grad(x, None)
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        assert needs_grad(None, dual)
+        with torch.no_grad():  # which leaves forward mode on
+            assert needs_grad(dual)
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_on_the_gpu():
+    """There is no kernel for tangents: refused, not dropped."""
+    x = torch.randn(3, 8, device='cuda:0')
+    one = torch.ones(8, device='cuda:0')
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for data, gamma, res in ((dual, one, None), (x, one, dual),
+                                 (x, torch.autograd.forward_ad.make_dual(
+                                     one, one), None)):
+            with pytest.raises(RuntimeError):
+                mx.nd.RMSNorm(*(mx.nd.from_torch(t) for t in (data, gamma)),
+                              residual=None if res is None
+                              else mx.nd.from_torch(res))
+        with pytest.raises(ValueError):
+            mx.nd.RMSNorm(mx.nd.from_torch(dual), mx.nd.from_torch(one),
+                          out_type='int8')
+        kv = mx.nd.from_torch(torch.randn(1, 4, 16, device='cuda:0'))
+        with pytest.raises(RuntimeError):
+            mx.nd.contrib.encdec_attention(mx.nd.from_torch(dual[None]), kv)
