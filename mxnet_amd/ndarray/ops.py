@@ -210,6 +210,9 @@ def RMSNorm(data, gamma, residual=None, axis=-1, eps=1e-6, out_type=None,
         ins = [data, gamma] + ([residual] if residual is not None else [])
         attrs = {'eps': repr(float(eps))}
         if out_type == 'int8':
+            from .. import _core
+            if _core.needs_grad([a._h for a in ins]):
+                raise ValueError(_nn.NO_INT8_GRADIENT)
             q, total, scale = _ninv('_contrib_rms_norm_int8', ins, attrs,
                                     nout=3)
             return [q, scale] + ([total] if residual is not None else [])

@@ -643,6 +643,10 @@ def needs_grad(*tensors):
         for t in tensors)
 
 
+NO_INT8_GRADIENT = ('RMSNorm: the int8 output has no gradient; call it outside '
+                    'autograd.record() or on detached arrays')
+
+
 def _rms_norm_check(x, gamma, residual, out_type):
     if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise TypeError(f'RMSNorm: float16, bfloat16 or float32 data, got '
@@ -677,9 +681,7 @@ def rms_norm(x, gamma, residual=None, axis=-1, eps=1e-6, out_type=None):
     _rms_norm_check(x, gamma, residual, out_type)
     if out_type == 'int8':
         if needs_grad(x, gamma, residual):
-            raise ValueError('RMSNorm: the int8 output has no gradient; call '
-                             'it outside autograd.record() or on detached '
-                             'arrays')
+            raise ValueError(NO_INT8_GRADIENT)
         if use_hip(x) and x.numel():
             q, h, scale = hip_required('rms_norm').rms_norm_fwd(
                 x, gamma, residual, eps, int8=True)

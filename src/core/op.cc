@@ -235,6 +235,31 @@ void Imperative::DropVariable(const NDArray& x) {
 
 void Imperative::ClearTape() { tape_.clear(); }
 
+// forward pass over the tape: leaves plus anything computed from them
+std::unordered_set<NDArray::Chunk*> Imperative::ChunksInNeed() const {
+  std::unordered_set<NDArray::Chunk*> need;
+  for (auto& kv : leaves_) need.insert(kv.first);
+  for (auto& node : tape_) {
+    bool any_in = false;
+    for (auto& in : node.inputs)
+      if (need.count(in.chunk_.get())) {
+        any_in = true;
+        break;
+      }
+    if (any_in)
+      for (auto& out : node.outputs) need.insert(out.chunk_.get());
+  }
+  return need;
+}
+
+bool Imperative::NeedsGrad(const std::vector<NDArray>& xs) const {
+  if (!recording_) return false;
+  const auto need = ChunksInNeed();
+  for (auto& x : xs)
+    if (need.count(x.chunk_.get())) return true;
+  return false;
+}
+
 void Imperative::Backward(const std::vector<NDArray>& ys,
                           const std::vector<NDArray>& y_grads,
                           bool retain_graph) {
@@ -259,21 +284,9 @@ void Imperative::Backward(const std::vector<NDArray>& ys,
            multi_copy_mode(src.dtype(), dst.dtype()) >= 0;
   };
 
-  // forward pass over the tape: which chunks require grad at all
-  // (leaves plus anything computed from them) — reference OpReqType
-  // kNullOp semantics; skips e.g. the input gradient of the first conv
-  std::unordered_set<NDArray::Chunk*> need;
-  for (auto& kv : leaves_) need.insert(kv.first);
-  for (auto& node : tape_) {
-    bool any_in = false;
-    for (auto& in : node.inputs)
-      if (need.count(in.chunk_.get())) {
-        any_in = true;
-        break;
-      }
-    if (any_in)
-      for (auto& out : node.outputs) need.insert(out.chunk_.get());
-  }
+  // which chunks require grad at all — reference OpReqType kNullOp
+  // semantics; skips e.g. the input gradient of the first conv
+  const std::unordered_set<NDArray::Chunk*> need = ChunksInNeed();
 
   std::unordered_map<NDArray::Chunk*, NDArray> grads;
   for (size_t i = 0; i < ys.size(); ++i) {

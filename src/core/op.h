@@ -13,6 +13,7 @@
 #include <functional>
 #include <string>
 #include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include "ndarray.h"
@@ -151,6 +152,9 @@ class Imperative {
   // eager reverse-mode sweep over the tape; clears the tape afterwards
   void Backward(const std::vector<NDArray>& ys,
                 const std::vector<NDArray>& y_grads, bool retain_graph);
+  // whether a gradient could flow into one of these: recording, and a leaf or
+  // computed from one on the tape
+  bool NeedsGrad(const std::vector<NDArray>& xs) const;
   void ClearTape();
   size_t TapeSize() const { return tape_.size(); }
 
@@ -162,6 +166,7 @@ class Imperative {
                       const std::vector<NDArray>& outputs);
 
  private:
+  std::unordered_set<NDArray::Chunk*> ChunksInNeed() const;
   static void PushOp(const OpEntry* op, const NodeAttrs& attrs,
                      const std::vector<NDArray>& inputs,
                      const std::vector<NDArray>& outputs);

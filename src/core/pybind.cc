@@ -288,6 +288,9 @@ PYBIND11_MODULE(_core, m) {
     py::gil_scoped_release rel;
     Imperative::Get()->Backward(ys, ygrads, retain);
   });
+  m.def("needs_grad", [](const std::vector<NDArray>& xs) {
+    return Imperative::Get()->NeedsGrad(xs);
+  });
   m.def("clear_tape", [] { Imperative::Get()->ClearTape(); });
   m.def("tape_size", [] { return Imperative::Get()->TapeSize(); });
 

@@ -463,3 +463,27 @@ def test_attention_over_no_keys(native, apart, device):
     assert out.shape == q.shape and not out.asnumpy().any()
     for v in ins:
         assert v.grad.shape == v.shape and not v.grad.asnumpy().any()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('on_native', [False, True])
+def test_int8_output_where_a_gradient_would_follow(on_native, device):
+    """Refused at the call on both runtimes, for marked arrays and for what
+    was computed of them; other calls within record() pass."""
+    prev = set_native(on_native)
+    try:
+        x, g = (mx.nd.array(np.ones(s, 'float32'), ctx=ctx(device))
+                for s in ((2, 16), (16,)))
+        assert x.is_native == on_native
+        free = mx.nd.array(np.ones((2, 16), 'float32'), ctx=ctx(device))
+        x.attach_grad()
+        with autograd.record():
+            for args in ((x, g, None), (x * 2, g, None), (free, g, x),
+                         (free, g, free + x)):
+                with pytest.raises(ValueError):
+                    mx.nd.RMSNorm(args[0], args[1], residual=args[2],
+                                  out_type='int8')
+            q = mx.nd.RMSNorm(free, g, residual=free * 2, out_type='int8')[0]
+        assert (q.asnumpy() == 127).all()
+    finally:
+        set_native(prev)
