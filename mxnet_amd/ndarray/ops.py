@@ -218,9 +218,17 @@ def RMSNorm(data, gamma, residual=None, axis=-1, eps=1e-6, out_type=None,
             return [q, scale] + ([total] if residual is not None else [])
         outs = _ninv('RMSNorm', ins, attrs, nout=3)
         return outs[:2] if residual is not None else outs[0]
-    out = _nn.rms_norm(_t(data), _t(gamma),
-                       _t(residual) if residual is not None else None, axis,
-                       eps, out_type)
+    args = (_t(data), _t(gamma), _t(residual) if residual is not None
+            else None, axis, eps, out_type)
+    if out_type is None:
+        out = _nn.rms_norm(*args)
+    else:
+        from .. import autograd as _ag
+        # (torch's grad mode is on outside record() too, where no gradient
+        # follows)
+        with torch.set_grad_enabled(torch.is_grad_enabled() and
+                                    _ag.is_recording()):
+            out = _nn.rms_norm(*args)
     return [NDArray(o) for o in out] if isinstance(out, tuple) \
         else NDArray(out)
 

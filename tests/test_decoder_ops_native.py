@@ -487,3 +487,26 @@ def test_int8_output_where_a_gradient_would_follow(on_native, device):
         assert (q.asnumpy() == 127).all()
     finally:
         set_native(prev)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('on_native', [False, True])
+def test_int8_output_of_a_trained_layer(on_native, device):
+    """Outside record() a layer's gamma and marked arrays give int8, as no
+    gradient follows."""
+    prev = set_native(on_native)
+    try:
+        layer = nn.RMSNorm()
+        layer.initialize(ctx=ctx(device))
+        x = mx.nd.array(np.ones((2, 16), 'float32'), ctx=ctx(device))
+        x.attach_grad()
+        with autograd.record():
+            loss = layer(x).sum()
+        loss.backward()
+        for pause in (False, True):
+            with autograd.pause() if pause else autograd.predict_mode():
+                q, s = mx.nd.RMSNorm(x, layer.gamma.data(), out_type='int8')
+            assert (q.asnumpy() == 127).all()
+            assert np.allclose(s.asnumpy(), 1 / 127)
+    finally:
+        set_native(prev)
