@@ -7,6 +7,7 @@ backward launches our HIP kernels, so ``record()`` maps to enabling grad
 mode and ``backward()`` to torch.autograd.backward — the gradient graph is
 executed asynchronously on the device's HIP streams exactly like forward.
 """
+import contextlib
 import threading
 
 import torch
@@ -107,15 +108,36 @@ def mark_variables(variables, gradients, grad_reqs='write'):
         v._t.grad = g._t
 
 
+class _InThisThread:
+    """torch's backward pass without its threads, and with the state that a
+    thread of its own would have: neither recording nor training."""
+
+    def __enter__(self):
+        self._threads = torch.autograd.set_multithreading_enabled(False)
+        self._was = set_recording(False), set_training(False)
+
+    def __exit__(self, *args):
+        set_recording(self._was[0])
+        set_training(self._was[1])
+        self._threads.__exit__(*args)
+
+
+def _only_device(index):
+    """Whether this process has worked on no GPU but that one."""
+    return all(i == index or not torch._C._cuda_hasPrimaryContext(i)
+               for i in range(torch.cuda.device_count()))
+
+
 def _engine_threads(tensors):
-    """Context for torch's backward pass.  Of heads on one GPU it runs in the
-    calling thread: handing each pass to the device's thread and waiting for
-    it costs about 50 us, and no second device could work meanwhile.  Heads
-    on several devices keep a thread for each."""
-    one = tensors and tensors[0].is_cuda and all(
-        t.device == tensors[0].device for t in tensors)
-    return torch.autograd.set_multithreading_enabled(
-        not one and torch._C._is_multithreading_enabled())
+    """Context for torch's backward pass.  Of heads on the only GPU of this
+    process it runs in the calling thread: handing each pass to the device's
+    thread and waiting for it costs about 50 us.  A process of several GPUs
+    keeps a thread for each, whose launches then do not wait for each other."""
+    if tensors and tensors[0].is_cuda and all(
+            t.device == tensors[0].device for t in tensors) \
+            and _only_device(tensors[0].get_device()):
+        return _InThisThread()
+    return contextlib.nullcontext()
 
 
 def backward(heads, head_grads=None, retain_graph=False, train_mode=True):
