@@ -7,6 +7,7 @@ from . import ops
 from .ndarray import concat, stack  # keep creation-module versions authoritative
 
 from . import contrib  # noqa: F401
+ops.contrib = contrib  # F.contrib of hybrid_forward, whose F is ops
 from . import random  # noqa: F401
 from . import sparse  # noqa: F401
 

@@ -3,14 +3,15 @@ neural-network ops over np-style arrays, plus np-mode switches."""
 import torch
 
 from .ndarray.ndarray import NDArray
-from .ndarray import ops as _ops
+from .ndarray import contrib as _contrib, ops as _ops
 from .util import set_np, reset_np, is_np_array  # noqa: F401
 
 __all__ = ['set_np', 'reset_np', 'is_np_array', 'softmax', 'log_softmax',
            'masked_softmax', 'relu', 'sigmoid', 'gelu', 'batch_norm',
            'layer_norm', 'rms_norm', 'fully_connected', 'convolution', 'pooling',
            'embedding', 'one_hot', 'pick', 'topk', 'batch_dot',
-           'sequence_mask', 'gamma', 'erf']
+           'sequence_mask', 'gamma', 'erf', 'encdec_attention',
+           'sample_tokens']
 
 softmax = _ops.softmax
 log_softmax = _ops.log_softmax
@@ -20,6 +21,8 @@ gelu = lambda x: NDArray(torch.nn.functional.gelu(x._t, approximate='tanh'))
 batch_norm = _ops.BatchNorm
 layer_norm = _ops.LayerNorm
 rms_norm = _ops.RMSNorm
+encdec_attention = _contrib.encdec_attention
+sample_tokens = _contrib.sample_tokens
 fully_connected = _ops.FullyConnected
 convolution = _ops.Convolution
 pooling = _ops.Pooling

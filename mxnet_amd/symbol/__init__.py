@@ -12,6 +12,8 @@ exactly like dmlc::Parameter printing.
 """
 import json
 
+from . import contrib
+
 __all__ = ['Symbol', 'var', 'Variable', 'Group', 'load', 'load_json']
 
 
@@ -240,6 +242,7 @@ _EVAL_TABLE = {
     '_minus_scalar': _scalar_op('_minus_scalar'),
     '_mul_scalar': _scalar_op('_mul_scalar'),
     '_div_scalar': _scalar_op('_div_scalar'),
+    **contrib.EVAL,
 }
 
 
