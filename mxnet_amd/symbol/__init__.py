@@ -322,6 +322,10 @@ def load_json(s):
         nodes.append(n)
     for n, jn in zip(nodes, g['nodes']):
         n.inputs = [(nodes[i], oi) for i, oi, _ in jn['inputs']]
+    rows = g.get('node_row_ptr')
+    if rows:
+        for i, n in enumerate(nodes):
+            n.num_outputs = rows[i + 1] - rows[i]
     heads = [(nodes[i], oi) for i, oi, _ in g['heads']]
     if len(heads) == 1:
         return Symbol(heads[0][0], heads[0][1])

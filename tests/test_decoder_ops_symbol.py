@@ -101,3 +101,14 @@ def test_nodes_with_every_argument(native, device, tmp_path):
             mask=feed['m']).asnumpy(), want[0].asnumpy())
     finally:
         set_native(prev)
+
+
+def test_saved_again_after_loading():
+    """A loaded graph knows how many outputs its nodes have."""
+    x, r, g = (mx.sym.var(n) for n in 'xrg')
+    y, h = mx.sym.RMSNorm(x, g, residual=r)
+    token, logp = mx.sym.contrib.sample_tokens(y, h, get_prob=True)
+    net = mx.sym.Group([y, h, token, logp])
+    again = mx.sym.load_json(net.tojson())
+    assert again.tojson() == net.tojson()
+    assert again[1].tojson() == logp.tojson()
