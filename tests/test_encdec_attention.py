@@ -435,3 +435,22 @@ def test_nothing_to_do_with_values_apart(size, layout, device):
         got = call(d, size, layout, grad=True)
         for g, name in zip(got, ('q', 'q', 'kv', 'values')):
             assert g.shape == d[name].shape and not g.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('B', [33, 64, 65, 130])
+@pytest.mark.parametrize('heads', [(2, 2), (3, 1), (6, 3)])
+@pytest.mark.parametrize('sq', [1, 40])
+def test_many_sequences_of_equal_and_unequal_lengths(sq, heads, B):
+    """Blocks take the sequences by their lengths, up to 64 of them: each is
+    written, once, with ties and empty ones among them."""
+    size = (B, *heads, sq, 70, 16)
+    g = torch.Generator().manual_seed(B)
+    some = torch.randint(0, 75, (B,), generator=g)
+    ties = torch.tensor([0, 7, 7, 64, 70])[torch.randint(0, 5, (B,),
+                                                         generator=g)]
+    for lengths in (some, ties, torch.full((B,), 33), torch.zeros(B),
+                    torch.arange(B) % 71, 70 - torch.arange(B) % 71):
+        d = make(size, torch.float16, 'cuda:0', seed=12,
+                 lengths=lengths.long().tolist())
+        check(call(d, size, 'NTC', grad=True), oracle(d, size, 'NTC'))
