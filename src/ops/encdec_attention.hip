@@ -37,9 +37,18 @@
 // waves of a block pass these phases together.  Single tokens are bound by HBM.
 //
 // Roundings to 16 bits, besides the results': the weights P and dS when they
-// become operands (half a step of each, as the inputs have; in fp16 below
-// 2^-14, where a row spreads over more than 16384 keys, half a step of 2^-24).
-// Maxima, sums, O, dQ, dK, dV and the split's partial results are 32 bits.
+// become operands (half a step of each, as the inputs have), and the output O
+// that the backward reads for dO . O (half a step of it, times dO).  Maxima,
+// sums, O, dQ, dK, dV and the split's partial results are 32 bits.
+//
+// fp16 holds no more than 2^-14 to 2^16 in full, and P and dS are smaller than
+// that in long rows and under small gradients.  So there the backward takes
+// them times 2^shift, and the factor out of the sums: 15, which P of at most 1
+// allows, as long as dS allows it too.  dQ looks at each tile's largest dS and
+// lowers its row's shift where it has to; dK and dV, whose sums go over rows,
+// take the lowest of their rows' shifts, which dQ leaves in the workspace.
+// (Of 1024 over 2048 keys of 64, dK was off by 23% under dO of 1e-5, where its
+// own rounding is 7%, and by 2.7% under 1e-4.)
 #include "ops_api.h"
 
 namespace mxcore {
@@ -74,6 +83,16 @@ template <> struct Mat<float> {
   }
 };
 
+// whether P and dS go times a power of two (see above)
+template <typename T>
+constexpr bool kShifted = std::is_same<T, _Float16>::value;
+constexpr float kMostDs = 0x1p15f;  // half of what fp16 holds
+// The shift goes into a row's log-sum, where that is small enough to take it
+// (and at 2^20, what float32 loses of a log-sum makes weights 4% wrong anyway);
+// a row's first shift
+constexpr float kMostLse = 0x1p20f;
+DEV_INLINE int first_shift(float lse) { return fabsf(lse) < kMostLse ? 15 : 0; }
+
 // Waves a SIMD: two where the `n` operands of a row take at most `most` bytes,
 // so that a wave's 256 registers hold them and their accumulators; else one.
 // The second hides most of the first's latencies: dK and dV of size 96 in 16
@@ -97,6 +116,8 @@ struct Att {
   const uint8_t* mask;   // [B, Sk], 0: masked, or null
   float* lse;            // [B, H, Sq] log2 of the row's sum, +inf: no key
   float* delta;          // [B, H, Sq]
+  int* shift;            // [B, Hk][splits of dQ][G, Sq], fp16 only
+  int dq_splits;
   float* part;           // partial results of a split, fp32
   int B, H, Hk, G, Sq, Sk, D;
   int nsplit;
@@ -767,6 +788,40 @@ __global__ __launch_bounds__(256) void att_join_kernel(Att a, int DP) {
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
+
+// A row's dS 2^shift of one tile: where the largest is over kMostDs, the shift
+// goes down until it lies between 2^13 and 2^14, for the row's sums too.  (An
+// infinity, of an infinite gradient, stays one and lowers nothing.)
+template <int DP, int KB>
+DEV_INLINE void lower_shift(float16_t (&s)[KB], float16_t (&acc)[DP / 32],
+                            float& lse) {
+  float t4[4] = {};
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        t4[j] = fmaxf(fmaxf(t4[j], fabsf(s[kb][i + j])),
+                      fabsf(s[kb][i + 4 + j]));
+  float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+  if (!__any(top > kMostDs)) return;
+  top = pair_max(top);
+  const int down = top > kMostDs && top < -kNegInf && fabsf(lse) < 2 * kMostLse
+                       ? ilogbf(top) - 13
+                       : 0;
+  const float f = ldexpf(1.f, -down);
+  lse += (float)down;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[kb][i] *= f;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[n][i] *= f;
+}
+
 // dQ: rows as in the forward, over all keys (or a split's).  61 us where the
 // forward takes 54, with 12 products for its 8; the row's dO . O costs one read
 // of its output here, and no launch.
@@ -801,7 +856,9 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
     qf[ks] = load_frag<T>(qr, ks, h, a.D, vec, row < M);
     gf[ks] = load_frag<T>(gr, ks, h, a.D, vec, row < M);
   }
-  const float lse = row < M ? a.lse[(long)bh * M + row] : -kNegInf;
+  float lse = row < M ? a.lse[(long)bh * M + row] : -kNegInf;
+  // (with the shift in it: exp2 then gives P 2^shift)
+  if constexpr (kShifted<T>) lse -= (float)first_shift(lse);
   // the row's dO . O, which dK and dV need too
   float delta = 0.f;
   {
@@ -848,17 +905,32 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
       for (int j = 0; j < 16; ++j)
         s[kb][j] =
             __builtin_amdgcn_exp2f(fmaf(s[kb][j], c, -lse)) * dp[kb][j];
+    if constexpr (kShifted<T>) lower_shift<DP, KB>(s, acc, lse);
     weigh<T, DP, KB>(lk[buf], s, acc, l);
     if (i + 1 < t1)
       kt.store(lk[buf ^ 1], lv[buf ^ 1], lkeep[buf ^ 1], i + 1);
     __syncthreads();
   });
   if (row >= M) return;
-  if (a.nsplit > 1)
+  float back = 1.f;
+  if constexpr (kShifted<T>) {
+    const float whole = a.lse[(long)bh * M + row];
+    const int shift =
+        fabsf(whole) < 4 * kMostLse ? (int)rintf(whole - lse) : 0;
+    back = ldexpf(1.f, -shift);
+    if (h == 0) a.shift[((long)bh * a.nsplit + split) * M + row] = shift;
+  }
+  if (a.nsplit > 1) {
+    if constexpr (kShifted<T>)
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[n][j] *= back;
     store_part<DP>(a.part + part_row(a, split, bh, row) * DP, acc, h);
-  else
-    store_row<T, DP>(q_row<T>(a.dq, a, b, hk, row), acc, a.scale, h, a.D,
-                     vec);
+  } else {
+    store_row<T, DP>(q_row<T>(a.dq, a, b, hk, row), acc, a.scale * back, h,
+                     a.D, vec);
+  }
 }
 
 // dK and dV: NW waves of 32 keys each over tiles of BM rows (or a split's).
@@ -890,6 +962,10 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2, 384))) void att_dkv_kerne
   const int t0 = (int)((long)tiles * split / a.nsplit);
   const int t1 = (int)((long)tiles * (split + 1) / a.nsplit);
 
+  // the rows' shifts, of which most launches have one a thread
+  const int shifts = kShifted<T> && t0 < t1 ? a.dq_splits * M : 0;
+  const int* ps = kShifted<T> ? a.shift + (long)bh * a.dq_splits * M : nullptr;
+  int least = t < shifts ? ps[t] : 15;
   typename Mat<T>::Frag kf[DP / 16], vf[DP / 16];
   const T* kr = keep ? row_ptr<T>(a.k, b, hk, key) : nullptr;
   const T* vr = keep ? row_ptr<T>(a.v, b, hk, key) : nullptr;
@@ -899,7 +975,6 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2, 384))) void att_dkv_kerne
     vf[ks] = load_frag<T>(vr, ks, h, a.D, vec, keep);
   }
   float16_t dk[DP / 32] = {}, dv[DP / 32] = {};
-
   using S = Stage<T, DP, BM, NT>;
   S sq, sg;
   const unsigned qo = S::offset(t, a.q.ss, a.D),
@@ -924,20 +999,47 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2, 384))) void att_dkv_kerne
       return q_row<T>(a.dout, a, b, hk, min(m0 + rr, M - 1));
     }, ok, t, a.D, vec);
   };
+  // Their lowest is the block's.  P takes it as far as it is not negative
+  // (small gradients), dS all of it
+  int shift = 0;
+  if (t0 < t1) fetch(t0);
+  if constexpr (kShifted<T>) {
+    __shared__ int lshift[NW];
+    for (int i = t + NT; i < shifts; i += NT) least = min(least, ps[i]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+      least = min(least, __shfl_xor(least, off, 64));
+    if (l == 0) lshift[t >> 6] = least;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NW; ++k) least = min(least, lshift[k]);
+    shift = __builtin_amdgcn_readfirstlane(least);
+  }
+  const int up = max(shift, 0);
+  auto scalar = [](float v) {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+  };
+  const float fup = scalar((float)up),
+              fdown = scalar(ldexpf(1.f, min(shift, 0)));
+  // (where it is negative, through V and dO . O: 16 products for each 32x32
+  // scores, or a branch, put registers into scratch memory)
+  if (kShifted<T> && shift < 0) {
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vf[ks][j] = (T)((float)vf[ks][j] * fdown);
+  }
   auto put = [&](int i, int buf) __attribute__((always_inline)) {
     const bool all = a.D == DP && (i + 1) * BM <= M;
     sq.store(lq[buf], t, all);
     sg.store(lg[buf], t, all);
     if (t < BM) {
       // a row past the end has a weight of exp2(-inf)
-      llse[buf][t] = i * BM + t < M ? rl : -kNegInf;
-      ldel[buf][t] = i * BM + t < M ? -rd : 0.f;
+      llse[buf][t] = i * BM + t < M ? rl - fup : -kNegInf;
+      ldel[buf][t] = i * BM + t < M ? -rd * fdown : 0.f;
     }
   };
-  if (t0 < t1) {
-    fetch(t0);
-    put(t0, 0);
-  }
+  if (t0 < t1) put(t0, 0);
   __syncthreads();
   in_turn(t0, t1, [&](int i, auto number) __attribute__((always_inline)) {
     constexpr int buf = decltype(number)::value;
@@ -994,6 +1096,10 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(2, 384))) void att_dkv_kerne
     for (int j = 0; j < 16; ++j) {
       const int k = k0 + 8 * (j / 4) + 4 * h + (j & 3), col = d * 32 + r;
       if (k >= a.Sk) continue;
+      if constexpr (kShifted<T>) {
+        dk[d][j] = ldexpf(dk[d][j], -shift);
+        dv[d][j] = ldexpf(dv[d][j], -up);
+      }
       if (!(kept >> (k - k0) & 1)) dk[d][j] = dv[d][j] = 0.f;
       if (a.nsplit > 1) {
         float* p = a.part +
@@ -1247,8 +1353,12 @@ void bwd(const LaunchCtx& lc, Att a, const Plan& p) {
   }
 }
 
-// the partial results behind delta start at 16 bytes
-int64_t align4(int64_t n) { return (n + 3) & ~(int64_t)3; }
+// Behind delta of each row, and its shift in each split of dQ, the backward's
+// partial results start at 16 bytes
+int64_t behind_rows(const Plan& p, int64_t rows, int dtype) {
+  const int64_t n = rows * (dtype == kFloat16 ? 1 + p.dq : 1);
+  return (n + 3) & ~(int64_t)3;
+}
 
 }  // namespace
 
@@ -1264,7 +1374,7 @@ std::vector<int64_t> encdec_attention_workspace(int64_t B, int64_t H,
   const int64_t dq = p.dq > 1 ? p.dq * rows * p.DP : 0;
   const int64_t dkv = p.dkv > 1 ? p.dkv * B * Hk * Sk * 2 * p.DP : 0;
   // the two splits of the backward use the workspace one after the other
-  return {fwd, align4(rows) + std::max(dq, dkv)};
+  return {fwd, behind_rows(p, rows, dtype) + std::max(dq, dkv)};
 }
 
 void encdec_attention_fwd_raw(const LaunchCtx& lc, const Arr& q,
@@ -1329,7 +1439,9 @@ void encdec_attention_bwd_raw(const LaunchCtx& lc, const Arr& dout,
   }
   a.lse = lse.data<float>();
   a.delta = work.data<float>();
-  a.part = work.data<float>() + align4(rows);
+  a.shift = (int*)(a.delta + rows);
+  a.dq_splits = p.dq;
+  a.part = a.delta + behind_rows(p, rows, q.dtype);
   DISPATCH_FLOAT_NATIVE(q.dtype, "encdec_attention backward",
                         [&] { bwd<scalar_t>(lc, a, p); });
   HIP_CHECK_LAST();
