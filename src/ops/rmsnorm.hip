@@ -441,19 +441,20 @@ __global__ __launch_bounds__(256) void rms_dgamma_long_kernel(
   partial[(long)blockIdx.y * C + c] = v;
 }
 
-// dgamma[c] = sum of the partials' column c: 32 columns a block, 32 threads a
-// column, eight reads of each on their way, always in the same order (512
-// partials of 768 columns: 3.2 us, bound by two rounds of latency)
+// dgamma[c] = sum of the partials' column c (rows of them lie `stride` apart):
+// 32 columns a block, 32 threads a column, eight reads of each on their way,
+// always in the same order (512 partials of 768 columns: 3.2 us, bound by two
+// rounds of latency)
 __global__ __launch_bounds__(1024) void rms_dgamma_kernel(
     const float* __restrict__ partial, float* __restrict__ dgamma, int nblk,
-    int C) {
+    int C, long stride) {
   __shared__ float part[32][33];
   const int col = threadIdx.x & 31, k = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + col;
   float v = 0.f;
   if (c < C) {
 #pragma unroll 8
-    for (int b = k; b < nblk; b += 32) v += partial[(long)b * C + c];
+    for (int b = k; b < nblk; b += 32) v += partial[b * stride + c];
   }
   part[k][col] = v;
   __syncthreads();
@@ -512,10 +513,10 @@ RowPlan plan_rows(long rows, int C, size_t size, bool aligned) {
       constexpr bool LOOSE = false; \
       LAUNCH(); \
     } \
-    return; \
+    RETURN; \
   }
 
-// LAUNCH sees VEC, TPR, NV and LOOSE as constants
+// LAUNCH sees VEC, TPR, NV and LOOSE as constants, RETURN follows it
 #define RMS_DISPATCH() \
   RMS_CASE(64, 1) \
   RMS_CASE(64, 2) \
@@ -554,6 +555,7 @@ void fwd_launch(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
   signed char* qp = INT8 ? (signed char*)y.ptr : nullptr;
   // a launch has fewer than 2^32 threads: 2^21 blocks of 1024 at most
   constexpr int VEC = 16 / sizeof(T);
+#define RETURN return
 #define LAUNCH()                                                            \
   constexpr int RPB = TPR < 256 ? 256 / TPR : 1;                            \
   for (long r0 = 0; r0 < rows; r0 += (1L << 21) * RPB) {                    \
@@ -570,6 +572,7 @@ void fwd_launch(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
   }
   RMS_DISPATCH()
 #undef LAUNCH
+#undef RETURN
   rms_fwd_long_kernel<T, RES, INT8>
       <<<(unsigned)std::min<long>(rows, 4096), 1024, 0, lc.stream>>>(
           x.data<T>(), res.data<T>(), gamma.data<float>(), yp, qp,
@@ -577,16 +580,18 @@ void fwd_launch(const LaunchCtx& lc, const Arr& x, const Arr& gamma,
           eps);
 }
 
+// returns the number of dgamma's partials, at most nblk
 template <typename T, bool DSUM>
-void bwd_launch(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
-                const Arr& h, const Arr& gamma, const Arr& rstd,
-                const Arr& dx, float* partial, int nblk) {
+int bwd_launch(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
+               const Arr& h, const Arr& gamma, const Arr& rstd, const Arr& dx,
+               float* partial, int nblk) {
   const int C = (int)h.size(-1);
   const long rows = h.numel() / C;
   RowPlan p = plan_rows(rows, C, sizeof(T),
                         aligned16({dy.ptr, dsum.ptr, h.ptr, gamma.ptr,
                                    dx.ptr}));
   constexpr int VEC = 16 / sizeof(T);
+#define RETURN return nblk
 #define LAUNCH()                                                          \
   rms_bwd_kernel<T, VEC, TPR, NV, LOOSE, DSUM>                            \
       <<<(unsigned)nblk, TPR < 256 ? 256 : TPR, 0, lc.stream>>>(          \
@@ -594,14 +599,18 @@ void bwd_launch(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
           rstd.data<float>(), dx.data<T>(), partial, rows, C)
   RMS_DISPATCH()
 #undef LAUNCH
+#undef RETURN
   rms_bwd_long_kernel<T, DSUM>
       <<<(unsigned)std::min<long>(rows, 4096), 1024, 0, lc.stream>>>(
           dy.data<T>(), dsum.data<T>(), h.data<T>(), gamma.data<float>(),
           rstd.data<float>(), dx.data<T>(), rows, C);
+  // (fewer than 2^32 threads: 2^23 blocks, or one for each 256 columns)
+  const int columns = (C + 255) / 256;
+  nblk = std::min(nblk, std::max(1, (1 << 23) / columns));
   rms_dgamma_long_kernel<T>
-      <<<dim3((unsigned)((C + 255) / 256), (unsigned)nblk), 256, 0,
-         lc.stream>>>(dy.data<T>(), h.data<T>(), rstd.data<float>(), partial,
-                      rows, C);
+      <<<dim3((unsigned)columns, (unsigned)nblk), 256, 0, lc.stream>>>(
+          dy.data<T>(), h.data<T>(), rstd.data<float>(), partial, rows, C);
+  return nblk;
 }
 
 }  // namespace
@@ -662,18 +671,24 @@ void rms_norm_bwd_raw(const LaunchCtx& lc, const Arr& dy, const Arr& dsum,
                dgamma.dtype == kFloat32 && dgamma.numel() == C &&
                partial.dtype == kFloat32 && partial.numel() >= nblk * C,
            "RMSNorm backward: statistics, dgamma or workspace too small");
+  int partials = 0;
   DISPATCH_FLOAT_NATIVE(h.dtype, "RMSNorm backward", [&] {
     if (rows == 0) return;
-    if (dsum.defined())
-      bwd_launch<scalar_t, true>(lc, dy, dsum, h, gamma, rstd, dx,
-                                 partial.data<float>(), (int)nblk);
-    else
-      bwd_launch<scalar_t, false>(lc, dy, dsum, h, gamma, rstd, dx,
-                                  partial.data<float>(), (int)nblk);
+    partials = dsum.defined()
+                   ? bwd_launch<scalar_t, true>(lc, dy, dsum, h, gamma, rstd,
+                                                dx, partial.data<float>(),
+                                                (int)nblk)
+                   : bwd_launch<scalar_t, false>(lc, dy, dsum, h, gamma, rstd,
+                                                 dx, partial.data<float>(),
+                                                 (int)nblk);
   });
-  rms_dgamma_kernel<<<(unsigned)((C + 31) / 32), 1024, 0, lc.stream>>>(
-      partial.data<float>(), dgamma.data<float>(), rows ? (int)nblk : 0,
-      (int)C);
+  // (fewer than 2^32 threads a launch: 2^26 columns)
+  for (int64_t c = 0; c < C; c += 1 << 26) {
+    const int64_t n = std::min<int64_t>(C - c, 1 << 26);
+    rms_dgamma_kernel<<<(unsigned)((n + 31) / 32), 1024, 0, lc.stream>>>(
+        partial.data<float>() + c, dgamma.data<float>() + c, partials, (int)n,
+        C);
+  }
   HIP_CHECK_LAST();
 }
 

@@ -472,3 +472,35 @@ def test_forward_mode_is_refused_on_the_gpu():
         kv = mx.nd.from_torch(torch.randn(1, 4, 16, device='cuda:0'))
         with pytest.raises(RuntimeError):
             mx.nd.contrib.encdec_attention(mx.nd.from_torch(dual[None]), kv)
+
+
+@pytest.mark.gpu
+def test_gradients_of_rows_past_2_27_columns():
+    """More columns than one launch of dgamma's last sum has threads for."""
+    rows, cols = 2, (1 << 27) + 3
+    g = torch.Generator(device='cuda:0').manual_seed(41)
+    x, dy = (torch.randn(rows, cols, device='cuda:0', generator=g).bfloat16()
+             for _ in range(2))
+    gamma = torch.rand(cols, device='cuda:0', generator=g) + 0.5
+    xs, gs = (mx.nd.from_torch(t.requires_grad_()) for t in (x, gamma))
+    with autograd.record():
+        y = mx.nd.RMSNorm(xs, gs)
+    dx, dg = (t.to_torch() for t in autograd.grad(
+        [y], [xs, gs], [mx.nd.from_torch(dy)]))
+    r = torch.rsqrt(torch.stack([t.double().square().mean() for t in x.detach()])
+                    + 1e-6)[:, None]
+    m = torch.stack([(a.double() * gamma.detach() * b).sum()
+                     for a, b in zip(dy, x.detach())])[:, None] * r / cols
+    for at in (slice(0, 1000), slice((1 << 26) - 500, (1 << 26) + 500),
+               slice(cols - 1000, cols)):
+        n = x.detach()[:, at].double() * r
+        a = dy[:, at].double()
+        # two products, each of two rounded factors, and their sum
+        within(dg[at], (a * n).sum(0), (a * n).abs().sum(0) * U32 * 6 + 1e-30)
+        t = a * gamma.detach()[at].double()
+        want = r * (t - n * m)
+        # (m is the mean of 2^27 terms: off by 2^-7 of their size at most, of
+        # which the row's sum of 2^17 in a thread has half a step each)
+        off = r * (t.abs() * 4 * U32 + n.abs() * (m.abs() * 8 * U32
+                                                  + 2.0 ** 17 * U32))
+        within(dx[:, at], want, off + want.abs() * 2.0 ** -8 + 1e-30)
