@@ -127,6 +127,10 @@ def _encdec_native(queries, keys_values, values, heads, kv_heads,
         raise ValueError(f'encdec_attention: layout must be NTC or TNC, got '
                          f'{layout!r}')
     heads = int(heads)
+    if heads > 0 and queries.shape[-1] // heads > 128 \
+            and queries.context.device_type == 'gpu':
+        raise ValueError(f'encdec_attention: head sizes up to 128 on the GPU, '
+                         f'got {queries.shape[-1] // heads}')
     more = [values, valid_length, mask]
     attrs = {'heads': str(heads),
              'kv_heads': str(heads if kv_heads is None else int(kv_heads)),

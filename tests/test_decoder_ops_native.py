@@ -510,3 +510,16 @@ def test_int8_output_of_a_trained_layer(on_native, device):
             assert np.allclose(s.asnumpy(), 1 / 127)
     finally:
         set_native(prev)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_large_heads(native, device):
+    """Refused at the call on the GPU, not where the result is read."""
+    q = arr(np.random.RandomState(15).randn(1, 2, 136).astype('float32'),
+            device)
+    if device == 'gpu':
+        with pytest.raises(ValueError):
+            mx.nd.contrib.encdec_attention(q, q, q, heads=1)
+    else:
+        assert mx.nd.contrib.encdec_attention(q, q, q, heads=1).shape == q.shape
+    assert mx.nd.contrib.encdec_attention(q, q, q, heads=2).shape == q.shape
