@@ -99,6 +99,20 @@ void* ArenaAlloc(const Context& c, size_t n, int lane) {
   return h.dptr;
 }
 
+namespace {
+// a kernel that is given another device's memory, or the host's, faults
+void CheckContexts(const OpEntry* op, const Context& ctx,
+                   const std::vector<NDArray>& arrays) {
+  for (auto& a : arrays) {
+    const Context c = a.ctx();
+    MX_CHECK(c == ctx || c.dev_type == Context::kCPUPinned ||
+                 (!c.is_gpu() && !ctx.is_gpu()),
+             "op '" << op->name << "' on " << ctx.str()
+                    << " is given an array on " << c.str());
+  }
+}
+}  // namespace
+
 void Imperative::PushOp(const OpEntry* op, const NodeAttrs& attrs,
                         const std::vector<NDArray>& inputs,
                         const std::vector<NDArray>& outputs) {
@@ -108,6 +122,9 @@ void Imperative::PushOp(const OpEntry* op, const NodeAttrs& attrs,
   const FCompute& fc = ctx.is_gpu() ? op->fcompute_gpu : op->fcompute_cpu;
   MX_CHECK(fc, "op '" << op->name << "' has no " << (ctx.is_gpu() ? "GPU" : "CPU")
                       << " implementation (native extension required)");
+
+  CheckContexts(op, ctx, inputs);
+  CheckContexts(op, ctx, outputs);
 
   std::vector<TBlob> in_blobs, out_blobs;
   in_blobs.reserve(inputs.size());
@@ -192,6 +209,7 @@ std::vector<NDArray> Imperative::Run(const OpEntry* op, const NodeAttrs& attrs,
     int id = (int)attrs.GetInt("__ctx_gpu__", -1);
     ctx = id >= 0 ? Context::GPU(id) : Context::CPU();
   }
+  CheckContexts(op, ctx, inputs);
   std::vector<NDArray> outputs;
   for (size_t i = 0; i < out_shapes.size(); ++i)
     outputs.emplace_back(out_shapes[i], ctx, out_dtypes[i]);

@@ -157,12 +157,12 @@ PYBIND11_MODULE(_core, m) {
 
   py::class_<NDArray>(m, "NDArray")
       .def(py::init([](const std::vector<int64_t>& shape, int dev_type,
-                       int dev_id, int dtype) {
+                       int dev_id, int dtype, bool delay_alloc) {
              return NDArray(TShape(shape.begin(), shape.end()),
-                            MakeCtx(dev_type, dev_id), dtype);
+                            MakeCtx(dev_type, dev_id), dtype, delay_alloc);
            }),
            py::arg("shape"), py::arg("dev_type") = 1, py::arg("dev_id") = 0,
-           py::arg("dtype") = 0)
+           py::arg("dtype") = 0, py::arg("delay_alloc") = false)
       .def_property_readonly("shape",
                              [](const NDArray& a) {
                                return std::vector<int64_t>(a.shape());
