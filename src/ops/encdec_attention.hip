@@ -912,6 +912,10 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1))) void att_dq_kernel(Att 
     __syncthreads();
   });
   if (row >= M) return;
+  if (lse == -kNegInf) {  // no key: zeros, also where dO is not finite
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) acc[n] = float16_t{};
+  }
   float back = 1.f;
   if constexpr (kShifted<T>) {
     const float whole = a.lse[(long)bh * M + row];

@@ -454,3 +454,22 @@ def test_many_sequences_of_equal_and_unequal_lengths(sq, heads, B):
         d = make(size, torch.float16, 'cuda:0', seed=12,
                  lengths=lengths.long().tolist())
         check(call(d, size, 'NTC', grad=True), oracle(d, size, 'NTC'))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('sq,sk', [(1, 70), (40, 70), (3, 3000)])
+def test_gradients_that_are_not_finite_beside_no_key(sq, sk, dtype, device):
+    """A row without a key is zeros whatever the inputs hold: so is its
+    gradient, and other sequences' gradients do not change."""
+    size = (3, 4, 2, sq, sk, 32)
+    d = make(size, dtype, device, seed=14, lengths=[sk, 0, sk], mask=True)
+    d['mask'][2] = False
+    want = call(d, size, 'NTC', grad=True)
+    for bad in (math.nan, math.inf):
+        e = dict(d, dout=d['dout'].clone())
+        e['dout'][1:] = bad
+        got = call(e, size, 'NTC', grad=True)
+        for g, w in zip(got, want):
+            assert torch.equal(g[0], w[0])
+            assert not g[1:].any() and not w[1:].any()
