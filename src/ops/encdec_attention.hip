@@ -24,13 +24,14 @@
 //
 // fp32 uses the fp32 matrix instructions (eight of k = 2 for one of k = 16).
 //
-// Measured at 4x16 heads, 1024 over 2048 keys, all of them kept, bf16:
-//   head size 64:   forward 61 us (560 TFLOP/s), backward 186 us (460)
-//   head size 96:   forward 79 us (650), backward 236 us (550)
-//   head size 128:  forward 101 us (680), backward 412 us (417)
-// and in fp32 at 2x16 heads, 1024 over 1024 keys of 64: 83 us (104), 270 us
-// (79).  A large library product reaches 1198 in bf16, 154 in fp32.  Long
-// 16-bit rows are bound by what surrounds the products: a wave spends 980
+// Measured at 4x16 heads, 1024 over 2048 keys, all of them kept, kernels back
+// to back, medians, bf16 (and backward in fp16, which scales P and dS):
+//   head size 64:   forward 57 us (600 TFLOP/s), backward 147 us (580; 156)
+//   head size 96:   forward 79 us (650), backward 233 us (550; 257)
+//   head size 128:  forward 88 us (780), backward 393 us (440; 385)
+// and in fp32 at 2x16 heads, 1024 over 1024 keys of 64: 82 us (105), 272 us
+// (79).  A large library product reaches 1198 in bf16, 154 in fp32.  As
+// scheduled here, what surrounds the products takes longest: a wave spends 980
 // cycles of vector instructions (32 exponentials of eight cycles, scaling,
 // sums, rounding) beside 517 of matrix instructions on 64 keys by 32 rows of
 // size 64; a wave's products hide about half of another's vector work, and the
@@ -96,9 +97,9 @@ DEV_INLINE int first_shift(float lse) { return fabsf(lse) < kMostLse ? 15 : 0; }
 // Waves a SIMD: two where the `n` operands of a row take at most `most` bytes,
 // so that a wave's 256 registers hold them and their accumulators; else one.
 // The second hides most of the first's latencies: dK and dV of size 96 in 16
-// bits are faster with two, of which 12 registers lie in scratch memory, than
-// with one (backward of 4x16 heads, 1024 over 2048 keys: 236 us, 332); of size
-// 128, where 59 would, with one (412 us, 527).
+// bits are faster with two, of which 12 registers (14 in fp16) lie in scratch
+// memory, than with one (backward of 4x16 heads, 1024 over 2048 keys in bf16:
+// 236 us, 332); of size 128, where 59 would, with one (412 us, 527).
 template <typename T, int DP>
 constexpr int waves(int n, int most = 256) {
   return n * DP * (int)sizeof(T) <= most ? 2 : 1;
@@ -658,7 +659,9 @@ __global__ __launch_bounds__(NW * 64, (waves<T, DP>(1, 384))) void att_fwd_kerne
 // its own part of LDS and without a barrier; the waves' results are joined at
 // the end.  Bound by HBM: 8x8 heads of four rows over up to 16384 keys of 128
 // in bf16 take 69 us (400 MB of kept keys: 5.8 TB/s) and the join 4.6; 32x16
-// heads over up to 512 keys of 64, 15 us (50 MB), which latency bounds.
+// heads over up to 512 keys of 64, 15 us (50 MB), which latency bounds.  In fp32
+// the two at full lengths take 237 us (4.5 TB/s; one wave a SIMD from size 65
+// on) and 31 (4.4).
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int BN>
 __global__ __launch_bounds__(256, (waves<T, DP>(1))) void att_token_kernel(Att a) {

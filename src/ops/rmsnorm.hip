@@ -244,7 +244,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(
 }
 
 // forward of rows that no register variant holds (over 32768 columns of 16
-// bits, 16384 of 32): the row is read again, from the cache
+// bits, 16384 of 32): the row is read again, from the cache, an element at a
+// time.  1024 rows of 65536 in bf16: forward 178 us (3.0 TB/s of what has to
+// be moved), backward 314 (1.7); in fp32 317 and 465.
 template <typename T, bool RES, bool INT8>
 __global__ __launch_bounds__(1024) void rms_fwd_long_kernel(
     const T* __restrict__ x, const T* __restrict__ res,
@@ -354,7 +356,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(
     }
     m = row_sum_f32<TPR>(m, red) / C;
     // (without this the compiler keeps the row's products for the loop below,
-    // in scratch memory where the registers do not hold them: 32768 columns)
+    // in scratch memory where the registers do not hold them: 32768 columns.
+    // Of four vectors of 16 bits, 5 to 9 registers still lie there.)
     if constexpr (!AHEAD) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
