@@ -113,13 +113,16 @@ class _InThisThread:
     thread of its own would have: neither recording nor training."""
 
     def __enter__(self):
-        self._threads = torch.autograd.set_multithreading_enabled(False)
-        self._was = set_recording(False), set_training(False)
+        s = _state()
+        self._was = (s.recording, s.training,
+                     torch._C._is_multithreading_enabled())
+        s.recording = s.training = False
+        torch._C._set_multithreading_enabled(False)
 
     def __exit__(self, *args):
-        set_recording(self._was[0])
-        set_training(self._was[1])
-        self._threads.__exit__(*args)
+        s = _state()
+        s.recording, s.training, threads = self._was
+        torch._C._set_multithreading_enabled(threads)
 
 
 def _only_device(index):
